@@ -144,6 +144,91 @@ int nrc_rope_freqs(float* out_host, size_t head_dim, float theta, float factor, 
 int nrc_rope_apply(float* x, size_t len, size_t head_dim, const float* freqs_host, size_t pos, int style,
                    void* stream);
 
+/* ---------------------------------------------------- serving over a paged KV cache */
+/* The reference keeps one contiguous cache per stream (crates/nr-model/src/infer.rs:319-350); these
+ * kernel-level entry points serve many sequences from one pool of pages, for hosts that schedule
+ * sequences themselves. Like the nr-tensor entry points they take device pointers of the current
+ * device, are asynchronous on `stream`, allocate nothing and may be captured into a CUDA graph.
+ * Strides count elements. A page id outside the pool, or a length or slot outside the table, is not
+ * followed: that position is left out, and nrc_sync_check returns NRC_ERR_DEVICE. */
+#define NRC_F32 0
+#define NRC_F16 1
+#define NRC_BF16 2
+
+/* Pages of K and V rows: the row of (page, offset, head) is head_dim contiguous values at
+ * page * page_stride + offset * pos_stride + head * head_stride, in k and in v alike. The position
+ * `slot` of sequence s lies in page table[s * table_stride + slot / page_size] at offset
+ * slot % page_size. k, v and the strides are multiples of 16 bytes; head_dim is 32, 64, 96 or 128. */
+typedef struct nrc_paged_kv {
+  void* k;
+  void* v;
+  const int32_t* table;
+  uint64_t n_pages;
+  int64_t page_stride, pos_stride, head_stride;
+  uint32_t page_size, n_kv_heads, head_dim, n_seqs, max_pages, table_stride;
+  int32_t dtype; /* NRC_F16 or NRC_BF16 */
+} nrc_paged_kv;
+
+/* Frequencies of a context stretched by `factor` (YaRN, Peng et al. 2023, arXiv:2309.00071): pairs
+ * that turn more than beta_fast times within original_context positions keep theta^(-2i/rot_dim),
+ * pairs that turn fewer than beta_slow times get it divided by factor, linearly mixed between.
+ * out_host: rot_dim/2 values; *mscale: 0.1 ln(factor) + 1, the factor on cos and sin (1 for
+ * factor <= 1). Computed on the host beside nrc_rope_freqs. */
+int nrc_rope_freqs_yarn(float* out_host, float* mscale, size_t rot_dim, float theta, float factor, float beta_fast,
+                        float beta_slow, float original_context);
+/* rope::apply (crates/nr-tensor/src/rope.rs:49-65) of new tokens at their own positions, and the
+ * append of infer.rs:536-551, over pages. For token t and pair i < rot_dim/2 of every head of q and k
+ * (style 0: values 2i, 2i+1; style 1: i, i + rot_dim/2; values from rot_dim on pass unchanged)
+ *   (a, b) -> mscale * (a cos - b sin, a sin + b cos),  angle = pos[t] * freqs_dev[i],
+ * the angle in 64 bits and the rest in f32, rounded once to the output's type (nearest even). q goes
+ * to q_out (q itself is allowed), k and v to slot[t] of sequence seq[t] (slot < 0: not cached).
+ * q: [tokens][n_heads][head_dim], k and v: [tokens][kv heads][head_dim], of `dtype`, with token and
+ * head strides; pos, seq, slot: int32 [tokens]. No two tokens of a call share (seq, slot). */
+int nrc_rope_append(const nrc_paged_kv* kv, void* q_out, int64_t qo_token, int64_t qo_head, const void* q,
+                    int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                    int64_t v_token, int64_t v_head, int dtype, size_t tokens, size_t n_heads, const float* freqs_dev,
+                    size_t rot_dim, float mscale, int style, const int32_t* pos, const int32_t* seq,
+                    const int32_t* slot, void* stream);
+/* Attention (infer.rs:553-572) of the newest n_new tokens of every sequence over its pages. lens[s]
+ * counts the cached positions, the new tokens' own among them; token i of n_new sees the positions
+ * before lens[s] - (n_new - 1 - i); one that sees nothing gets zeros. Per query head
+ *   out = sum_t p_t V_t,  p = softmax(scale * q . K_t),
+ * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into as
+ * many cache-typed parts as hold all the bits of `dtype`. q and out: [n_seqs][n_new][n_heads]
+ * [head_dim] of `dtype`, each with sequence, token and head strides. weights (or NULL): f32
+ * [n_seqs][kv heads][weights_len]; the weight that a position received from all the query heads of
+ * the KV head and all new tokens is added to it. max_len: no sequence is longer (0: the table's
+ * width). workspace: nrc_attn_paged_workspace bytes, 16-byte aligned, used by one call at a time. */
+int nrc_attn_paged_workspace(const nrc_paged_kv* kv, size_t n_new, size_t n_heads, int with_weights, size_t max_len,
+                             size_t* out_bytes);
+int nrc_attn_paged(const nrc_paged_kv* kv, void* out, int64_t o_seq, int64_t o_token, int64_t o_head, const void* q,
+                   int64_t q_seq, int64_t q_token, int64_t q_head, int dtype, size_t n_new, size_t n_heads,
+                   const int32_t* lens, float scale, float* weights, size_t weights_len, size_t max_len,
+                   void* workspace, size_t workspace_bytes, void* stream);
+/* Eviction: every sequence longer than `budget` keeps, for each KV head, its first `sinks` and latest
+ * `recent` positions and the others of largest weight (ties: the earlier one; NaN counts as the
+ * smallest), budget in all. The kept rows of K and V move to the slots 0..budget-1 in their order, in
+ * place. kept: int32 [n_seqs][kv heads][budget], the old slots in ascending order, -1 behind a
+ * shorter sequence's; new_lens[s] = min(lens[s], budget); new_weights[s][h] = the weights of the kept
+ * positions, then zeros. weights and new_weights: f32 [n_seqs][kv heads][weights_len].
+ * new_lens == lens and new_weights == weights are allowed. sinks + recent <= budget <= weights_len. */
+int nrc_kv_evict(const nrc_paged_kv* kv, int32_t* kept, int32_t* new_lens, float* new_weights, const int32_t* lens,
+                 const float* weights, size_t weights_len, size_t budget, size_t recent, size_t sinks, void* stream);
+/* Drafted tokens against the target, beside nrc_sample: row i of p is the target's distribution
+ * after the first i drafted tokens. Token i (below n_draft[s]) is taken while
+ *   u[i] * q_i(draft_i) < p_i(draft_i)
+ * (exact in 64 bits); at the first refusal a the next token is drawn from max(p_a - q_a, 0), or,
+ * when every draft was taken, from p_a: the first index whose running sum, in 64 bits, exceeds
+ * u[n_max] times the whole sum (p_a itself where the difference leaves nothing; token 0 where that
+ * holds nothing positive either; NaN counts as nothing). tokens[s] = the a taken drafts, the drawn
+ * token, then -1; accepted[s] = a. p: [n_seqs][n_max + 1][vocab], q: [n_seqs][n_max][vocab] (NULL:
+ * each draft was certain, q = 1 at it), of `dtype`, with sequence and token strides; draft: int32
+ * [n_seqs][n_max] (an id outside the vocabulary is refused); u: f32 [n_seqs][n_max + 1] in [0, 1);
+ * n_draft: int32 [n_seqs] or NULL (n_max everywhere); tokens: int32 [n_seqs][n_max + 1]. */
+int nrc_verify_draft(int32_t* tokens, int32_t* accepted, const void* p, int64_t p_seq, int64_t p_token, const void* q,
+                     int64_t q_seq, int64_t q_token, int dtype, size_t n_seqs, size_t n_max, size_t vocab,
+                     const int32_t* draft, const float* u, const int32_t* n_draft, void* stream);
+
 /* ----------------------------------------------------------------- nr-model */
 
 typedef struct nrc_model nrc_model;

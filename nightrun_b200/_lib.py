@@ -49,6 +49,14 @@ class SynthCfg(C.Structure):
                 ("name", C.c_char * 48)]
 
 
+class PagedKVDesc(C.Structure):
+    """nrc_paged_kv."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "table")] + [("n_pages", C.c_uint64)] + \
+               [(n, C.c_int64) for n in ("page_stride", "pos_stride", "head_stride")] + \
+               [(n, C.c_uint32) for n in ("page_size", "n_kv_heads", "head_dim", "n_seqs", "max_pages",
+                                          "table_stride")] + [("dtype", C.c_int32)]
+
+
 def synth_cfg(cfg):
     s = SynthCfg()
     for k, _ in SynthCfg._fields_:
@@ -62,7 +70,7 @@ def synth_cfg(cfg):
 _LIB = None
 
 # (name, restype, argtypes) of every exported entry point.
-P, S, F, I, U32, U64 = C.c_void_p, C.c_size_t, C.c_float, C.c_int, C.c_uint32, C.c_uint64
+P, S, F, I, U32, U64, L = C.c_void_p, C.c_size_t, C.c_float, C.c_int, C.c_uint32, C.c_uint64, C.c_int64
 SIGNATURES = [
     ("nrc_last_error", C.c_char_p, []),
     ("nrc_version", I, []),
@@ -91,6 +99,12 @@ SIGNATURES = [
     ("nrc_sample", I, [P, S, F, F, P, P, P]),
     ("nrc_rope_freqs", I, [P, S, F, F, F, F, F]),
     ("nrc_rope_apply", I, [P, S, S, P, S, I, P]),
+    ("nrc_rope_freqs_yarn", I, [P, P, S, F, F, F, F, F]),
+    ("nrc_rope_append", I, [P] + [P, L, L] * 4 + [I, S, S, P, S, F, I, P, P, P, P]),
+    ("nrc_attn_paged_workspace", I, [P, S, S, I, S, C.POINTER(S)]),
+    ("nrc_attn_paged", I, [P, P, L, L, L, P, L, L, L, I, S, S, P, F, P, S, S, P, S, P]),
+    ("nrc_kv_evict", I, [P, P, P, P, P, P, S, S, S, S, P]),
+    ("nrc_verify_draft", I, [P, P, P, L, L, P, L, L, I, S, S, S, P, P, P, P]),
     ("nrc_model_load", I, [P, S, I, I, C.POINTER(P)]),
     ("nrc_gguf_to_nrm", I, [P, S, P, S, C.POINTER(S)]),
     ("nrc_model_load_gguf", I, [P, S, I, C.POINTER(P)]),

@@ -13,6 +13,7 @@
 #include "mma.cuh"
 #include "nrcuda.h"
 #include "ops.cuh"
+#include "paged.cuh"
 #include "sample.cuh"
 
 using namespace nrc;
@@ -349,10 +350,17 @@ int nrc_sync_check(void* stream) {
   if (rc) return rc;
   unsigned err = 0;
   if (cudaMemcpy(&err, sc.err, 4, cudaMemcpyDeviceToHost) != cudaSuccess) return nrc_fail_api(NRC_ERR_CUDA, "read error word");
+  unsigned paged = 0, attn = 0;
+  if (paged_take_errors(&paged) != cudaSuccess || paged_attn_take_errors(&attn) != cudaSuccess)
+    return nrc_fail_api(NRC_ERR_CUDA, "read error word");
   if (err) {
     cudaMemset(sc.err, 0, 4);
     return nrc_fail_api(NRC_ERR_DEVICE, "kernel wait expired (error bits 0x%x)", err);
   }
+  if (paged | attn)
+    return nrc_fail_api(NRC_ERR_DEVICE, "%s (error bits 0x%x)",
+                        (paged | attn) & ERR_BAD_PAGE ? "a page id outside the pool" : "a length, sequence or slot outside the table",
+                        paged | attn);
   return NRC_OK;
 }
 

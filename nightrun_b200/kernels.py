@@ -11,6 +11,8 @@ import ctypes as C
 import torch
 
 from ._lib import check, lib
+from .paged import (PagedKV, attn_paged, attn_paged_workspace, evict, rope_append,  # noqa: F401
+                    rope_freqs_yarn, verify_draft)
 
 Q8_0_BYTES, Q4K_BYTES, Q6K_BYTES, Q8K_BYTES = 34, 144, 210, 292
 QK8_0, QK_K = 32, 256
