@@ -10,7 +10,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libnrcuda.so")
 SOURCES = ["gemv.cu", "mma.cu", "ops.cu", "attn.cu", "synth.cu", "engine.cu", "api.cu", "noalloc.cu", "sample.cu", "tp.cu", "mma_kq.cu", "gguf.cu",
-           "paged.cu", "paged_attn.cu", "verify.cu", "paged_api.cu"]
+           "paged.cu", "paged_attn.cu", "paged_attn_f16_1.cu", "paged_attn_f16_2.cu", "paged_attn_bf16_1.cu",
+           "paged_attn_bf16_2.cu", "paged_attn_bf16_3.cu", "verify.cu", "paged_api.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 

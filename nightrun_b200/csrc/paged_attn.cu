@@ -1,106 +1,81 @@
-// Attention of the newest tokens of many sequences over a paged KV cache.
-#include "paged.cuh"
+// Host side of the paged attention: the variant, the schedule and the workspace's layout.
+#include "paged_attn.cuh"
 
 namespace nrc {
 namespace {
 
 __device__ unsigned g_attn_err;
 
-constexpr int PA_THREADS = 128, PA_WARPS = PA_THREADS / 32;
+using pattn::Plan;
 
-// One CTA per (KV head, sequence): for each query row one pass over the positions, a warp per
-// position, with the running maximum and sum of the softmax; where weights are wanted a second pass
-// adds them in row order.
-template <int PER>  // head_dim / 32
-__global__ void __launch_bounds__(PA_THREADS) k_paged_attn(const PagedAttnArgs a) {
-  constexpr int HD = 32 * PER;
-  __shared__ float sm[PA_WARPS], sl[PA_WARPS], so[PA_WARPS][HD];
-  const uint32_t h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t gqa = a.n_heads / a.kv.n_kv_heads;
-  const int32_t raw = a.lens[b];
-  uint32_t len = raw < 0 ? 0u : (uint32_t)raw;
-  const uint32_t most = a.weights && a.weights_len < a.max_len ? a.weights_len : a.max_len;
-  if (raw < 0 || len > most) {
-    if (threadIdx.x == 0) atomicOr(&g_attn_err, ERR_BAD_SLOT);
-    len = raw < 0 ? 0u : most;
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;  // only a size asked for without a device
+  return n;
+}
+
+// Fills the plan and returns the workspace's bytes; `base` null: sizes only.
+size_t make_plan(Plan& p, int* nt, uint8_t* base) {
+  const nrc_paged_kv& kv = p.a.kv;
+  p.gqa = p.a.n_heads / kv.n_kv_heads;
+  p.rows = p.gqa * p.a.n_new;
+  *nt = p.rows <= 8 ? 1 : p.rows <= 16 || kv.head_dim > pattn::MAX_HD_NT4 ? 2 : 4;
+  const uint32_t cols = 8 * *nt;
+  p.row_blocks = (p.rows + cols - 1) / cols;
+  const uint64_t items = (uint64_t)kv.n_seqs * kv.n_kv_heads * p.row_blocks;
+  const uint32_t units = (p.a.max_len + pattn::UNIT - 1) / pattn::UNIT;
+  p.min_units = 4;
+  p.direct = units <= p.min_units && items <= 0x7fffffffu;
+  if (p.direct) {
+    p.blocks = (uint32_t)items;
+  } else {
+    const uint64_t all = items * units, resident = (uint64_t)sm_count() * (*nt == 1 ? 3 : 2);
+    const uint64_t want = (all + p.min_units - 1) / p.min_units;
+    p.blocks = (uint32_t)(want < resident ? want : resident);
   }
-  const uint16_t* kb = static_cast<const uint16_t*>(a.kv.k) + (int64_t)h * a.kv.head_stride;
-  const uint16_t* vb = static_cast<const uint16_t*>(a.kv.v) + (int64_t)h * a.kv.head_stride;
-  for (uint32_t r = 0; r < gqa * a.n_new; r++) {
-    const uint32_t tok = r / gqa, head = h * gqa + r % gqa;
-    const int64_t sees = (int64_t)len - (a.n_new - 1 - tok);
-    const uint32_t n = sees > 0 ? (uint32_t)sees : 0u;
-    float q[PER], acc[PER], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      q[i] = load_as_f32(a.q, (int64_t)b * a.q_seq + (int64_t)tok * a.q_token + (int64_t)head * a.q_head + lane + 32 * i,
-                         a.dtype);
-      acc[i] = 0.0f;
-    }
-    auto score = [&](uint32_t t, int64_t* row) {
-      *row = paged_row(a.kv, b, t);
-      if (*row < 0) {
-        if (lane == 0) atomicOr(&g_attn_err, ERR_BAD_PAGE);
-        return -INFINITY;
-      }
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < PER; i++) s += q[i] * load_as_f32(kb, *row + lane + 32 * i, a.kv.dtype);
-      return warp_sum(s) * a.scale;
-    };
-    for (uint32_t t = warp; t < n; t += PA_WARPS) {
-      int64_t row;
-      const float s = score(t, &row);
-      if (row < 0 || s == -INFINITY) continue;
-      const float mn = fmaxf(m, s), old = expf(m - mn), p = expf(s - mn);
-      l = l * old + p;
-#pragma unroll
-      for (int i = 0; i < PER; i++) acc[i] = acc[i] * old + p * load_as_f32(vb, row + lane + 32 * i, a.kv.dtype);
-      m = mn;
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int i = 0; i < PER; i++) so[warp][lane + 32 * i] = acc[i];
-    __syncthreads();
-    float mx = -INFINITY, total = 0.0f;
-    for (int w = 0; w < PA_WARPS; w++) mx = fmaxf(mx, sm[w]);
-    for (int w = 0; w < PA_WARPS; w++) total += sl[w] == 0.0f ? 0.0f : sl[w] * expf(sm[w] - mx);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    for (int d = threadIdx.x; d < HD; d += PA_THREADS) {
-      float o = 0.0f;
-      for (int w = 0; w < PA_WARPS; w++) o += sl[w] == 0.0f ? 0.0f : so[w][d] * expf(sm[w] - mx);
-      store_from_f32(a.out, (int64_t)b * a.o_seq + (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, a.dtype,
-                     o * inv);
-    }
-    if (a.weights) {
-      float* wr = a.weights + ((size_t)b * a.kv.n_kv_heads + h) * a.weights_len;
-      for (uint32_t t = warp; t < n; t += PA_WARPS) {  // a position stays with its warp in every row
-        int64_t row;
-        const float s = score(t, &row);
-        if (lane == 0 && row >= 0 && s != -INFINITY) wr[t] += expf(s - mx) * inv;
-      }
-    }
-    __syncthreads();
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return base ? base + here : nullptr;
+  };
+  if (!p.direct) {
+    p.cut = reinterpret_cast<int4*>(take(sizeof(int4) * p.blocks));
+    p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * 2 * p.blocks * cols));
+    p.part_o = reinterpret_cast<float*>(take(sizeof(float) * 2 * p.blocks * cols * kv.head_dim));
   }
+  p.lse = nullptr;
+  if (p.a.weights) p.lse = reinterpret_cast<float*>(take(sizeof(float) * kv.n_seqs * kv.n_kv_heads * p.rows));
+  return at;
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const nrc_paged_kv&, uint32_t, uint32_t, bool, uint32_t) { return 0; }
+size_t paged_attn_workspace(const nrc_paged_kv& kv, uint32_t n_new, uint32_t n_heads, bool weights, uint32_t max_len) {
+  Plan p{};
+  p.a.kv = kv;
+  p.a.n_new = n_new;
+  p.a.n_heads = n_heads;
+  p.a.max_len = max_len;
+  p.a.weights = weights ? reinterpret_cast<float*>(1) : nullptr;
+  int nt;
+  return make_plan(p, &nt, nullptr);
+}
 
 cudaError_t paged_attn_run(const PagedAttnArgs& a, cudaStream_t s) {
-  PagedAttnArgs aa = a;
-  void* args[] = {&aa};
-  const void* fn = nullptr;
-  switch (a.kv.head_dim) {
-    case 32: fn = (const void*)k_paged_attn<1>; break;
-    case 64: fn = (const void*)k_paged_attn<2>; break;
-    case 96: fn = (const void*)k_paged_attn<3>; break;
-    case 128: fn = (const void*)k_paged_attn<4>; break;
-    default: return cudaErrorInvalidValue;
-  }
-  return launch_kernel(fn, dim3(a.kv.n_kv_heads, a.kv.n_seqs), dim3(PA_THREADS), 0, s, false, args);
+  Plan p{};
+  p.a = a;
+  int nt;
+  make_plan(p, &nt, static_cast<uint8_t*>(a.workspace));
+  void* err = nullptr;
+  if (cudaError_t e = cudaGetSymbolAddress(&err, g_attn_err)) return e;
+  p.err = static_cast<unsigned*>(err);
+  // Parts of the cache's type that hold the bits of q's (and out's) type.
+  if (a.kv.dtype == NRC_F16) return a.dtype == NRC_F32 ? paged_attn_f16_2(p, nt, s) : paged_attn_f16_1(p, nt, s);
+  return a.dtype == NRC_F32   ? paged_attn_bf16_3(p, nt, s)
+         : a.dtype == NRC_F16 ? paged_attn_bf16_2(p, nt, s)
+                              : paged_attn_bf16_1(p, nt, s);
 }
 
 cudaError_t paged_attn_take_errors(unsigned* bits) {
