@@ -17,6 +17,12 @@ int cuda_rc(cudaError_t e, const char* what) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned4(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
+  auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & 3; };
+  return !(low(a) | low(b) | low(c) | low(d));
+}
+// A pointer that holds whole values of the type.
+inline bool aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == NRC_F32 ? 3 : 1)) == 0; }
 inline bool float_type(int t) { return t == NRC_F32 || t == NRC_F16 || t == NRC_BF16; }
 
 int check_kv(const nrc_paged_kv* kv) {
@@ -24,7 +30,7 @@ int check_kv(const nrc_paged_kv* kv) {
   if (kv->dtype != NRC_F16 && kv->dtype != NRC_BF16) return nrc_fail_api(NRC_ERR_INVALID, "cache type %d", kv->dtype);
   if (kv->head_dim < 32 || kv->head_dim > 128 || kv->head_dim % 32)
     return nrc_fail_api(NRC_ERR_INVALID, "head_dim %u (32, 64, 96 or 128)", kv->head_dim);
-  if (kv->page_size == 0 || kv->n_kv_heads == 0 || kv->n_kv_heads > 65535)
+  if (kv->page_size == 0 || kv->n_kv_heads == 0 || kv->n_kv_heads > 16384)
     return nrc_fail_api(NRC_ERR_INVALID, "page size %u, %u KV heads", kv->page_size, kv->n_kv_heads);
   if (kv->n_seqs > 65535) return nrc_fail_api(NRC_ERR_INVALID, "%u sequences (65535 at most)", kv->n_seqs);
   if (kv->n_pages > 0x7fffffffull || (uint64_t)kv->max_pages * kv->page_size > 0x7fffffffull)
@@ -32,6 +38,7 @@ int check_kv(const nrc_paged_kv* kv) {
   if (kv->table_stride < kv->max_pages) return nrc_fail_api(NRC_ERR_INVALID, "table rows overlap");
   if (kv->n_pages && (!kv->k || !kv->v)) return nrc_fail_api(NRC_ERR_INVALID, "null pages");
   if (kv->n_seqs && kv->max_pages && !kv->table) return nrc_fail_api(NRC_ERR_INVALID, "null table");
+  if (!aligned4(kv->table)) return nrc_fail_api(NRC_ERR_INVALID, "table is not 4-byte aligned");
   if (!aligned16(kv->k) || !aligned16(kv->v) || kv->page_stride % 8 || kv->pos_stride % 8 || kv->head_stride % 8)
     return nrc_fail_api(NRC_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
   return NRC_OK;
@@ -69,10 +76,13 @@ int nrc_rope_append(const nrc_paged_kv* kv, void* q_out, int64_t qo_token, int64
   if (!float_type(dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", dtype);
   if (style != 0 && style != 1) return nrc_fail_api(NRC_ERR_INVALID, "style %d", style);
   if (rot_dim % 2 || rot_dim > kv->head_dim) return nrc_fail_api(NRC_ERR_INVALID, "rot_dim %zu", rot_dim);
-  if (tokens > 0x7fffffff || n_heads > 65535) return nrc_fail_api(NRC_ERR_INVALID, "shape too large");
+  if (tokens > 0x7fffffff || n_heads > 16384) return nrc_fail_api(NRC_ERR_INVALID, "shape too large");
   if (tokens == 0) return NRC_OK;
   if ((n_heads && (!q_out || !q)) || !k || !v || !pos || !seq || !slot || (rot_dim && !freqs))
     return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if (!aligned(q, dtype) || !aligned(k, dtype) || !aligned(v, dtype) || !aligned(q_out, dtype) ||
+      !aligned4(freqs, pos, seq, slot))
+    return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
   RopeAppendArgs a{};
   a.kv = *kv;
   a.q_out = q_out;
@@ -89,7 +99,7 @@ int nrc_rope_append(const nrc_paged_kv* kv, void* q_out, int64_t qo_token, int64
 static int check_attn(const nrc_paged_kv* kv, size_t n_new, size_t n_heads, size_t* max_len) {
   if (int rc = check_kv(kv)) return rc;
   if (n_new == 0 || n_new > NRC_MAX_BATCH) return nrc_fail_api(NRC_ERR_INVALID, "%zu new tokens (1..64)", n_new);
-  if (n_heads == 0 || n_heads % kv->n_kv_heads || n_heads > 65535)
+  if (n_heads == 0 || n_heads % kv->n_kv_heads || n_heads > 16384)
     return nrc_fail_api(NRC_ERR_INVALID, "%zu query heads over %u KV heads", n_heads, kv->n_kv_heads);
   const size_t slots = (size_t)kv->max_pages * kv->page_size;
   if (*max_len == 0 || *max_len > slots) *max_len = slots;
@@ -115,6 +125,8 @@ int nrc_attn_paged(const nrc_paged_kv* kv, void* out, int64_t o_seq, int64_t o_t
     return nrc_fail_api(NRC_ERR_INVALID, "weights of length %zu", weights_len);
   if (kv->n_seqs == 0) return NRC_OK;
   if (!out || !q || !lens) return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if (!aligned(out, dtype) || !aligned(q, dtype) || !aligned4(lens, weights))
+    return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
   const size_t need = paged_attn_workspace(*kv, (uint32_t)n_new, (uint32_t)n_heads, weights != nullptr, (uint32_t)max_len);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return nrc_fail_api(NRC_ERR_INVALID, "workspace of %zu bytes, 16-byte aligned: %zu needed",
@@ -146,6 +158,8 @@ int nrc_kv_evict(const nrc_paged_kv* kv, int32_t* kept, int32_t* new_lens, float
   if (kv->n_seqs == 0) return NRC_OK;
   if ((budget && !kept) || !new_lens || !lens || (weights_len && (!weights || !new_weights)))
     return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if (!aligned4(kept, new_lens, new_weights) || !aligned4(lens, weights))
+    return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not 4-byte aligned");
   EvictArgs a{};
   a.kv = *kv;
   a.kept = kept, a.new_lens = new_lens, a.new_weights = new_weights;
@@ -159,9 +173,11 @@ int nrc_verify_draft(int32_t* tokens, int32_t* accepted, const void* p, int64_t 
                      const int32_t* draft, const float* u, const int32_t* n_draft, void* stream) {
   if (!float_type(dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", dtype);
   if (n_max > NRC_MAX_BATCH - 1) return nrc_fail_api(NRC_ERR_INVALID, "%zu drafted tokens (63 at most)", n_max);
-  if (vocab == 0 || vocab > 0x7fffffff || n_seqs > 0x7fffffff) return nrc_fail_api(NRC_ERR_INVALID, "bad shape");
+  if (vocab == 0 || vocab > 0x7fffffff || n_seqs > 0xfffffff) return nrc_fail_api(NRC_ERR_INVALID, "bad shape");
   if (n_seqs == 0) return NRC_OK;
   if (!tokens || !accepted || !p || !u || (n_max && !draft)) return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if (!aligned(p, dtype) || !aligned(q, dtype) || !aligned4(tokens, accepted, draft, u) || !aligned4(n_draft))
+    return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
   VerifyArgs a{};
   a.tokens = tokens, a.accepted = accepted;
   a.p = p, a.q = q;

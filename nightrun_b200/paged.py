@@ -85,7 +85,7 @@ class PagedKV:
         _need(not any(x % 8 for x in (ps, rs, hs)) and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0,
               "pages and their strides must be multiples of 16 bytes")
         _need(self.n_pages < 2 ** 31 and self.max_pages * self.page_size < 2 ** 31 and self.n_seqs < 65536
-              and self.n_kv_heads < 65536, "cache too large")
+              and self.n_kv_heads <= 16384, "cache too large")
         self.desc = PagedKVDesc(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), self.n_pages, ps, rs, hs,
                                 self.page_size, self.n_kv_heads, self.head_dim, self.n_seqs, self.max_pages,
                                 table.stride(0) if self.n_seqs > 1 else self.max_pages, _DTYPES[k_pages.dtype])

@@ -27,7 +27,7 @@ def desc(**kw):
 BAD_CACHES = [dict(dtype=0), dict(dtype=7), dict(head_dim=48), dict(head_dim=160), dict(head_dim=0), dict(page_size=0),
               dict(n_kv_heads=0), dict(n_seqs=70000), dict(max_pages=2 ** 28, table_stride=2 ** 28), dict(table_stride=1),
               dict(k=FAKE + 8), dict(v=FAKE + 2), dict(page_stride=2052), dict(pos_stride=132), dict(head_stride=68),
-              dict(n_pages=2 ** 31), dict(k=None), dict(table=None)]
+              dict(n_pages=2 ** 31), dict(k=None), dict(table=None), dict(table=FAKE + 2), dict(n_kv_heads=16385)]
 
 
 def rope(L, kv, dtype=0, tokens=4, heads=4, rot=64, style=1, q=FAKE, freqs=FAKE, pos=FAKE):
@@ -57,7 +57,8 @@ def test_every_operator_refuses_a_bad_cache(L, bad):
 
 def test_rope_append_refusals(L):
     for kw in (dict(dtype=3), dict(dtype=-1), dict(style=2), dict(rot=63), dict(rot=66), dict(q=None), dict(freqs=None),
-               dict(pos=None), dict(tokens=2 ** 31), dict(heads=70000)):
+               dict(pos=None), dict(tokens=2 ** 31), dict(heads=70000), dict(q=FAKE + 2), dict(q=FAKE + 1, dtype=1),
+               dict(pos=FAKE + 1), dict(freqs=FAKE + 2)):
         assert rope(L, desc(), **kw) == -1, kw
         assert L.nrc_last_error()
     assert rope(L, desc(), tokens=0) == 0  # nothing to do, nothing launched
@@ -68,7 +69,7 @@ def test_attn_paged_refusals(L):
     assert L.nrc_attn_paged_workspace(desc(), 1, 4, 0, 0, C.byref(need)) == 0
     for kw in (dict(new=0), dict(new=65), dict(heads=3), dict(heads=0), dict(dtype=5), dict(scale=math.nan),
                dict(scale=math.inf), dict(weights=FAKE, wlen=0), dict(weights=FAKE, wlen=2 ** 31), dict(q=None),
-               dict(lens=None)):
+               dict(lens=None), dict(lens=FAKE + 2), dict(q=FAKE + 2), dict(weights=FAKE + 2, wlen=32)):
         kw = dict(ws=FAKE, wsb=1 << 40) | kw
         assert attn(L, desc(), **kw) == -1, kw
     if need.value:
@@ -82,14 +83,15 @@ def test_attn_paged_refusals(L):
 
 def test_evict_refusals(L):
     for kw in (dict(budget=33), dict(wlen=4), dict(recent=9), dict(recent=8, sinks=1), dict(sinks=7), dict(kept=None),
-               dict(weights=None), dict(wlen=2 ** 31, budget=2)):
+               dict(weights=None), dict(wlen=2 ** 31, budget=2), dict(kept=FAKE + 1), dict(weights=FAKE + 2)):
         assert evict(L, desc(), **kw) == -1, kw
     assert evict(L, desc(), wlen=64, budget=40) == -1  # more than the table's 32 positions
     assert evict(L, desc(n_seqs=0)) == 0
 
 
 def test_verify_draft_refusals(L):
-    for kw in (dict(dtype=4), dict(n=64), dict(vocab=0), dict(vocab=2 ** 31), dict(p=None), dict(draft=None)):
+    for kw in (dict(dtype=4), dict(n=64), dict(vocab=0), dict(vocab=2 ** 31), dict(p=None), dict(draft=None),
+               dict(p=FAKE + 1, dtype=2), dict(p=FAKE + 2), dict(draft=FAKE + 2), dict(seqs=2 ** 28)):
         assert verify(L, **kw) == -1, kw
     assert verify(L, seqs=0) == 0
 
