@@ -7,67 +7,160 @@ namespace {
 __device__ unsigned g_paged_err;
 
 // ------------------------------------------------------------ rotary append
-// One thread per (token, head, pair): the pair's angle pos * freq is formed in 64 bits and reduced
-// to a fraction of a turn there (a far position's angle has no correct digit left in 32 bits past
-// 2^24 turns), its sine and cosine in f32.
-__global__ void k_rope_append_paged(const RopeAppendArgs a) {
-  const uint32_t hd = a.kv.head_dim, half_hd = hd / 2, nh = a.n_heads + 2 * a.kv.n_kv_heads;
-  const size_t total = (size_t)a.tokens * nh * half_hd;
-  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
-    const uint32_t pr = i % half_hd;
-    const size_t th = i / half_hd;
-    const uint32_t h = th % nh, t = th / nh;
-    const uint32_t half = a.rot_dim / 2;
-    const bool rotate = pr < half && h < a.n_heads + a.kv.n_kv_heads;
-    // Pairs from rot_dim on are neighbours that pass unchanged.
-    uint32_t ia, ib;
-    if (pr < half && a.style == 1)
-      ia = pr, ib = pr + half;
-    else
-      ia = 2 * pr, ib = 2 * pr + 1;
-    const bool is_q = h < a.n_heads, is_k = !is_q && h < a.n_heads + a.kv.n_kv_heads;
-    const uint32_t kh = is_q ? 0 : is_k ? h - a.n_heads : h - a.n_heads - a.kv.n_kv_heads;
+// y = mscale R(pos f) x on pairs of q and k, v as it is. One pass over the values: bound by HBM for many
+// tokens, by latency for few.
+//
+// A block takes one token and up to ROPE_THREADS items of 2 W values of its heads: W neighbouring pairs
+// (interleaved), or W values of the first half with their W partners in the second. Its first threads form the
+// token's angles once for all heads, in 64 bits, reduced to a fraction of a turn there (in 32 bits a far
+// position's angle has lost all its digits after 2^24 turns), sine and cosine in f32; the values are
+// already on their way then. W is the widest access (16 bytes at most) that every pointer, stride and, for
+// halves, half the rotated width allow.
+constexpr int ROPE_THREADS = 128;
+
+template <int BYTES>
+struct Bits;
+template <>
+struct Bits<16> { using T = uint4; };
+template <>
+struct Bits<8> { using T = uint2; };
+template <>
+struct Bits<4> { using T = uint32_t; };
+template <>
+struct Bits<2> { using T = uint16_t; };
+
+// W values of type DT at element offset i, in registers of the widest access.
+template <int DT, int W>
+NRC_DEV void load_values(float (&x)[W], const void* p, int64_t i) {
+  constexpr int SIZE = DT == NRC_F32 ? 4 : 2;
+  using T = typename Bits<SIZE * W>::T;
+  const T raw = *reinterpret_cast<const T*>(static_cast<const uint8_t*>(p) + i * SIZE);
+#pragma unroll
+  for (int e = 0; e < W; e++) x[e] = load_as_f32(&raw, e, DT);
+}
+template <int DT, int W>
+NRC_DEV void store_values(const float (&x)[W], void* p, int64_t i) {
+  constexpr int SIZE = DT == NRC_F32 ? 4 : 2;
+  using T = typename Bits<SIZE * W>::T;
+  T raw;
+#pragma unroll
+  for (int e = 0; e < W; e++) store_from_f32(&raw, e, DT, x[e]);
+  *reinterpret_cast<T*>(static_cast<uint8_t*>(p) + i * SIZE) = raw;
+}
+
+template <int DT, int W>
+__global__ void __launch_bounds__(ROPE_THREADS) k_rope_append_paged(const RopeAppendArgs a) {
+  __shared__ float2 cs[64];  // cosine and sine of each pair (head_dim <= 128)
+  const uint32_t t = blockIdx.x, hd = a.kv.head_dim, half = a.rot_dim / 2, hk = a.kv.n_kv_heads;
+  const uint32_t per_head = hd / (2 * W), item = blockIdx.y * ROPE_THREADS + threadIdx.x;
+  const uint32_t hh = item / per_head, c = item - hh * per_head;
+  const bool live = hh < a.n_heads + 2 * hk;
+  const bool is_q = hh < a.n_heads, is_k = !is_q && hh < a.n_heads + hk;
+  const uint32_t h = is_q ? hh : is_k ? hh - a.n_heads : hh - a.n_heads - hk;
+  // Halves: the first half / W items of a head pair its halves, the others hold what is not rotated.
+  const bool turned = (is_q || is_k) && (a.style == 0 ? c * 2 * W < a.rot_dim : c * W < half);
+  uint32_t i0 = 2 * W * c, i1 = i0 + W;
+  if (a.style == 1 && c * W < half) {
+    i0 = c * W;
+    i1 = i0 + half;
+  }
+  float x[W], y[W];
+  int32_t slot = -1, seq = 0;
+  if (live) {
     const void* src = is_q ? a.q : is_k ? a.k : a.v;
-    const int64_t so = is_q   ? (int64_t)t * a.q_token + (int64_t)h * a.q_head
-                       : is_k ? (int64_t)t * a.k_token + (int64_t)kh * a.k_head
-                              : (int64_t)t * a.v_token + (int64_t)kh * a.v_head;
-    float x = load_as_f32(src, so + ia, a.dtype), y = load_as_f32(src, so + ib, a.dtype);
-    if (rotate) {
-      const double turns = (double)a.pos[t] * (double)a.freqs[pr] * 0.15915494309189533577;
-      float c, s;
-      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-      c *= a.mscale;
-      s *= a.mscale;
-      const float u = x * c - y * s, w = x * s + y * c;
-      x = u;
-      y = w;
-    }
-    if (is_q) {
-      const int64_t o = (int64_t)t * a.qo_token + (int64_t)h * a.qo_head;
-      store_from_f32(a.q_out, o + ia, a.dtype, x);
-      store_from_f32(a.q_out, o + ib, a.dtype, y);
+    const int64_t from = is_q   ? (int64_t)t * a.q_token + (int64_t)h * a.q_head
+                         : is_k ? (int64_t)t * a.k_token + (int64_t)h * a.k_head
+                                : (int64_t)t * a.v_token + (int64_t)h * a.v_head;
+    load_values<DT, W>(x, src, from + i0);
+    load_values<DT, W>(y, src, from + i1);
+    if (!is_q) slot = a.slot[t], seq = a.seq[t];
+  }
+  for (uint32_t i = threadIdx.x; i < half; i += ROPE_THREADS) {
+    const double turns = (double)a.pos[t] * (double)a.freqs[i] * 0.15915494309189533577;
+    float sn, co;
+    sincospif(2.0f * (float)(turns - rint(turns)), &sn, &co);
+    cs[i] = make_float2(co * a.mscale, sn * a.mscale);
+  }
+  __syncthreads();
+  if (!live) return;
+  if (turned) {
+    if (a.style == 1) {
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        const float2 r = cs[i0 + e];
+        const float u = x[e] * r.x - y[e] * r.y;
+        y[e] = x[e] * r.y + y[e] * r.x;
+        x[e] = u;
+      }
+    } else if (W == 1) {
+      const float2 r = cs[c];
+      const float u = x[0] * r.x - y[0] * r.y;
+      y[0] = x[0] * r.y + y[0] * r.x;
+      x[0] = u;
     } else {
-      const int32_t slot = a.slot[t], seq = a.seq[t];
-      if (slot < 0) continue;
-      if (seq < 0 || (uint32_t)seq >= a.kv.n_seqs || (uint32_t)slot / a.kv.page_size >= a.kv.max_pages) {
-        atomicOr(&g_paged_err, ERR_BAD_SLOT);
-        continue;
+#pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const uint32_t px = W * c + e / 2, py = px + W / 2;
+        if (px < half) {
+          const float2 r = cs[px];
+          const float u = x[e] * r.x - x[(e + 1) % W] * r.y;
+          x[(e + 1) % W] = x[e] * r.y + x[(e + 1) % W] * r.x;
+          x[e] = u;
+        }
+        if (py < half) {
+          const float2 r = cs[py];
+          const float u = y[e] * r.x - y[(e + 1) % W] * r.y;
+          y[(e + 1) % W] = y[e] * r.y + y[(e + 1) % W] * r.x;
+          y[e] = u;
+        }
       }
-      const int64_t row = paged_row(a.kv, seq, slot);
-      if (row < 0) {
-        atomicOr(&g_paged_err, ERR_BAD_PAGE);
-        continue;
-      }
-      void* dst = is_k ? a.kv.k : a.kv.v;
-      const int64_t o = row + (int64_t)kh * a.kv.head_stride;
-      store_from_f32(dst, o + ia, a.kv.dtype, x);
-      store_from_f32(dst, o + ib, a.kv.dtype, y);
     }
+  }
+  if (is_q) {
+    const int64_t to = (int64_t)t * a.qo_token + (int64_t)h * a.qo_head;
+    store_values<DT, W>(x, a.q_out, to + i0);
+    store_values<DT, W>(y, a.q_out, to + i1);
+    return;
+  }
+  if (slot < 0) return;
+  if (seq < 0 || (uint32_t)seq >= a.kv.n_seqs || (uint32_t)slot / a.kv.page_size >= a.kv.max_pages) {
+    atomicOr(&g_paged_err, ERR_BAD_SLOT);
+    return;
+  }
+  const int64_t row = paged_row(a.kv, seq, slot);
+  if (row < 0) {
+    atomicOr(&g_paged_err, ERR_BAD_PAGE);
+    return;
+  }
+  void* dst = is_k ? a.kv.k : a.kv.v;
+  const int64_t to = row + (int64_t)h * a.kv.head_stride;
+  if (a.kv.dtype == NRC_F16) {
+    store_values<NRC_F16, W>(x, dst, to + i0);
+    store_values<NRC_F16, W>(y, dst, to + i1);
+  } else {
+    store_values<NRC_BF16, W>(x, dst, to + i0);
+    store_values<NRC_BF16, W>(y, dst, to + i1);
   }
 }
 
+template <int DT, int W>
+cudaError_t launch_rope(const RopeAppendArgs& a, cudaStream_t s) {
+  const uint32_t items = (a.n_heads + 2 * a.kv.n_kv_heads) * (a.kv.head_dim / (2 * W));
+  k_rope_append_paged<DT, W><<<dim3(a.tokens, (items + ROPE_THREADS - 1) / ROPE_THREADS), ROPE_THREADS, 0, s>>>(a);
+  return cudaGetLastError();
+}
+template <int DT>
+cudaError_t launch_rope_w(const RopeAppendArgs& a, uint32_t w, cudaStream_t s) {
+  if constexpr (DT != NRC_F32)
+    if (w == 8) return launch_rope<DT, 8>(a, s);
+  return w >= 4 ? launch_rope<DT, 4>(a, s) : w == 2 ? launch_rope<DT, 2>(a, s) : launch_rope<DT, 1>(a, s);
+}
+
 // ------------------------------------------------------------ eviction
-constexpr int EV_THREADS = 1024;
+// The kept positions of a (sequence, KV head): the largest key that `want` weights reach, found by three radix passes,
+// then one pass in position order. Bound by latency (a few passes over a row that stays in L1 and L2) for few
+// rows, and beside the move of the kept rows, bound by HBM, for many.
+constexpr int EV_THREADS = 1024, EV_BINS = 2048, EV_EACH = 4;
 
 // Weights ordered as unsigned keys: larger weight, larger key; both zeros alike; NaN the smallest.
 NRC_DEV uint32_t weight_key(float v) {
@@ -76,19 +169,7 @@ NRC_DEV uint32_t weight_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-NRC_DEV uint32_t block_sum(uint32_t v, uint32_t* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  uint32_t s = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) s += red[w];
-  return s;
-}
-
-// Exclusive prefix sum of v over the block; *total its sum.
+// Exclusive prefix sum of v over the EV_THREADS threads; *total its sum. Two barriers.
 NRC_DEV uint32_t block_scan(uint32_t v, uint32_t* red, uint32_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t x = v;
@@ -100,13 +181,15 @@ NRC_DEV uint32_t block_scan(uint32_t v, uint32_t* red, uint32_t* total) {
   __syncthreads();
   if (lane == 31) red[warp] = x;
   __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
-    if (w < warp) before += red[w];
-    all += red[w];
+  uint32_t w = red[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  *total = all;
-  return before + x - v;
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const uint32_t before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+  return (warp ? before : 0) + x - v;
 }
 
 // The sequence's length, at most what its table and the weights hold.
@@ -121,116 +204,177 @@ NRC_DEV uint32_t evict_len(const EvictArgs& a, uint32_t b) {
   return (uint32_t)raw;
 }
 
-// One CTA per (sequence, KV head): the key of the last position kept by its weight, found bit by bit
-// from the top (the largest key that at least `want` keys reach); then one pass in position order
-// writes the kept slots and their weights.
 __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs a) {
-  __shared__ uint32_t red[32];
-  const uint32_t h = blockIdx.x, b = blockIdx.y;
+  __shared__ uint32_t red[32], hist[EV_BINS], found[2];
+  const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const size_t row = (size_t)b * a.kv.n_kv_heads + h;
   const uint32_t n = evict_len(a, b);
   const float* w = a.weights + row * a.weights_len;
   float* nw = a.new_weights + row * a.weights_len;
   int32_t* kept = a.kept + row * a.budget;
-  const uint32_t lo = a.sinks, hi = n > a.budget ? n - a.recent : n;  // chosen by weight: [lo, hi)
-  uint32_t key = 0, ties = 0;
-  if (n > a.budget) {
-    const uint32_t want = a.budget - a.sinks - a.recent;
-    if (want == 0) {
-      key = 0xffffffffu;  // no weight's key
-    } else {
-      for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t probe = key | (1u << bit);
-        uint32_t c = 0;
-        for (uint32_t t = lo + threadIdx.x; t < hi; t += EV_THREADS) c += weight_key(w[t]) >= probe;
-        if (block_sum(c, red) >= want) key = probe;
+  const bool all = n <= a.budget;
+  const uint32_t lo = a.sinks, hi = all ? n : n - a.recent;  // chosen by weight: [lo, hi)
+  // Positions of [lo, hi) whose key is above `key` are kept, and the first `ties` of those that equal it.
+  uint32_t key = 0xffffffffu, ties = 0;  // no weight's key
+  if (!all && a.budget > a.sinks + a.recent) {
+    uint32_t need = a.budget - a.sinks - a.recent, prefix = 0, mask = 0;
+    for (int pass = 0; pass < 3; pass++) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t bins = pass < 2 ? 2048u : 1024u;
+      for (uint32_t i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 8
+      for (uint32_t t = lo + tid; t < hi; t += EV_THREADS) {
+        const uint32_t k = weight_key(w[t]);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
       }
-      uint32_t c = 0;
-      for (uint32_t t = lo + threadIdx.x; t < hi; t += EV_THREADS) c += weight_key(w[t]) > key;
-      ties = want - block_sum(c, red);
+      __syncthreads();
+      // Bins from the largest on, two a thread: where the count reaches `need`.
+      const uint32_t c0 = hist[EV_BINS - 1 - 2 * tid], c1 = hist[EV_BINS - 2 - 2 * tid];
+      uint32_t total;
+      const uint32_t above = block_scan(c0 + c1, red, &total);
+      if (above < need && above + c0 + c1 >= need) {
+        const bool first = above + c0 >= need;
+        found[0] = EV_BINS - 1 - 2 * tid - (first ? 0 : 1);
+        found[1] = need - above - (first ? 0 : c0);
+      }
+      __syncthreads();
+      prefix |= found[0] << shift;
+      mask |= (bins - 1) << shift;
+      need = found[1];
     }
+    key = prefix;
+    ties = need;
   }
-  uint32_t at = 0, tied = 0;
-  for (uint32_t t0 = 0; t0 < n; t0 += EV_THREADS) {
-    const uint32_t t = t0 + threadIdx.x;
-    bool keep = false, tie = false;
-    float v = 0.0f;
-    if (t < n) {
-      v = w[t];
-      if (n <= a.budget || t < lo || t >= hi) {
-        keep = true;
-      } else {
-        const uint32_t k = weight_key(v);
-        keep = k > key;
-        tie = k == key;
+  uint32_t above = 0, tied = 0;
+  for (uint32_t t0 = 0; t0 < n; t0 += EV_THREADS * EV_EACH) {
+    float v[EV_EACH];
+    uint32_t keep = 0, tie = 0;
+    const uint32_t t1 = t0 + tid * EV_EACH;
+#pragma unroll
+    for (int e = 0; e < EV_EACH; e++) {
+      const uint32_t t = t1 + e;
+      if (t < n) {
+        v[e] = w[t];
+        const uint32_t k = weight_key(v[e]);
+        const bool fixed = all || t < lo || t >= hi;
+        keep |= (fixed || k > key ? 1u : 0u) << e;
+        tie |= (!fixed && k == key ? 1u : 0u) << e;
       }
     }
-    uint32_t all;
-    const uint32_t nth = tied + block_scan(tie, red, &all);
-    tied += all;
-    keep = keep || (tie && nth < ties);
-    const uint32_t to = at + block_scan(keep, red, &all);  // its barriers: w[t0..] is read before nw is written
-    at += all;
-    if (keep) {
-      kept[to] = (int32_t)t;
-      nw[to] = v;
+    uint32_t sum;
+    // Its barriers stand between the reads of these positions and the writes below (new_weights may be weights).
+    const uint32_t before = block_scan((uint32_t)__popc(keep) << 16 | (uint32_t)__popc(tie), red, &sum);
+    uint32_t g = above + (before >> 16), q = tied + (before & 0xffffu);
+#pragma unroll
+    for (int e = 0; e < EV_EACH; e++) {
+      const bool is_tie = (tie >> e) & 1, kp = ((keep >> e) & 1) || (is_tie && q < ties);
+      const uint32_t to = g + min(q, ties);
+      if (kp) {
+        kept[to] = (int32_t)(t1 + e);
+        nw[to] = v[e];
+      }
+      g += (keep >> e) & 1;
+      q += is_tie;
     }
+    above += sum >> 16;
+    tied += sum & 0xffffu;
   }
-  for (uint32_t i = at + threadIdx.x; i < a.budget; i += EV_THREADS) kept[i] = -1;
+  const uint32_t count = above + min(tied, ties);
+  for (uint32_t i = count + tid; i < a.budget; i += EV_THREADS) kept[i] = -1;
   __syncthreads();
-  for (uint32_t i = at + threadIdx.x; i < a.weights_len; i += EV_THREADS) nw[i] = 0.0f;
+  for (uint32_t i = count + tid; i < a.weights_len; i += EV_THREADS) nw[i] = 0.0f;
+  pdl_trigger();
 }
 
-// One CTA per (sequence, KV head, K or V): rows move down to their new slots in ascending order.
-// Slot i receives slot kept[i] >= i, so a batch of rows that is read whole before it is written
-// overwrites nothing that a later batch reads.
-__global__ void __launch_bounds__(EV_THREADS) k_evict_move(const EvictArgs a) {
-  const uint32_t h = blockIdx.x, b = blockIdx.y;
+// Rows move down to their new slots in ascending order. Slot i receives slot kept[i] >= i, so a batch of rows that is
+// read whole before it is written overwrites nothing that a later batch reads; one block takes all the rows
+// of a (sequence, KV head, K or V), or a column of them where there are too few of those to fill the GPU.
+// Bound by HBM: a batch keeps MV_EACH 16-byte pieces per thread in flight.
+constexpr int MV_THREADS = 256, MV_EACH = 8;
+
+__global__ void __launch_bounds__(MV_THREADS) k_evict_move(const EvictArgs a, const uint32_t pieces) {
+  pdl_wait();
+  const uint32_t cols = a.kv.head_dim / 8 / pieces, h = blockIdx.x / cols, b = blockIdx.y;
+  // new_lens may be lens: only this thread reads that element here.
+  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+    const uint32_t n = evict_len(a, b);
+    a.new_lens[b] = (int32_t)(n < a.budget ? n : a.budget);
+  }
+  if (a.budget == 0) return;
   const int32_t* kept = a.kept + ((size_t)b * a.kv.n_kv_heads + h) * a.budget;
-  uint16_t* base = static_cast<uint16_t*>(blockIdx.z ? a.kv.v : a.kv.k) + (int64_t)h * a.kv.head_stride;
-  const uint32_t vecs = a.kv.head_dim / 8, rows = EV_THREADS / vecs;
-  const uint32_t r = threadIdx.x / vecs, c = threadIdx.x % vecs;
-  for (uint32_t i0 = 0; i0 < a.budget; i0 += rows) {
-    const uint32_t i = i0 + r;
-    const int32_t src = r < rows && i < a.budget ? kept[i] : -1;
-    uint4 x;
-    int64_t to = -1;
-    if (src >= 0) {
-      if ((uint32_t)src != i) {
-        const int64_t from = paged_row(a.kv, b, src);
-        to = paged_row(a.kv, b, i);
-        if (from < 0 || to < 0) {
+  const int32_t end = kept[a.budget - 1];
+  if (end < 0 || (uint32_t)end == a.budget - 1) return;  // every row is where it belongs
+  uint16_t* base = static_cast<uint16_t*>(blockIdx.z ? a.kv.v : a.kv.k) + (int64_t)h * a.kv.head_stride +
+                   (blockIdx.x % cols) * pieces * 8 + (threadIdx.x % pieces) * 8;
+  const uint32_t rows = MV_THREADS / pieces, r = threadIdx.x / pieces;
+  // The rows of one batch: slot i0 + e * rows + r for each e.
+  auto locate = [&](uint32_t i0, int64_t (&from)[MV_EACH], int64_t (&to)[MV_EACH]) {
+    int32_t src[MV_EACH];
+#pragma unroll
+    for (int e = 0; e < MV_EACH; e++) {
+      const uint32_t i = i0 + e * rows + r;
+      src[e] = r < rows && i < a.budget ? kept[i] : -1;
+      if ((uint32_t)src[e] == i) src[e] = -1;
+    }
+#pragma unroll
+    for (int e = 0; e < MV_EACH; e++) {
+      from[e] = to[e] = -1;
+      if (src[e] >= 0) {
+        from[e] = paged_row(a.kv, b, src[e]);
+        to[e] = paged_row(a.kv, b, i0 + e * rows + r);
+        if (from[e] < 0 || to[e] < 0) {
           atomicOr(&g_paged_err, ERR_BAD_PAGE);
-          to = -1;
-        } else {
-          x = reinterpret_cast<const uint4*>(base + from)[c];
+          from[e] = -1;
         }
       }
     }
+  };
+  int64_t from[MV_EACH], to[MV_EACH];
+  locate(0, from, to);
+  for (uint32_t i0 = 0; i0 < a.budget; i0 += rows * MV_EACH) {
+    uint4 x[MV_EACH];
+    int64_t into[MV_EACH];
+#pragma unroll
+    for (int e = 0; e < MV_EACH; e++) {
+      into[e] = from[e] >= 0 ? to[e] : -1;
+      if (from[e] >= 0) x[e] = *reinterpret_cast<const uint4*>(base + from[e]);
+    }
+    locate(i0 + rows * MV_EACH, from, to);
     __syncthreads();
-    if (to >= 0) reinterpret_cast<uint4*>(base + to)[c] = x;
-  }
-  // new_lens may be lens: only this thread still reads that element.
-  if (h == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
-    const uint32_t n = evict_len(a, b);
-    a.new_lens[b] = (int32_t)(n < a.budget ? n : a.budget);
+#pragma unroll
+    for (int e = 0; e < MV_EACH; e++)
+      if (into[e] >= 0) *reinterpret_cast<uint4*>(base + into[e]) = x[e];
   }
 }
 
 }  // namespace
 
 cudaError_t rope_append_paged_run(const RopeAppendArgs& a, cudaStream_t s) {
-  const size_t total = (size_t)a.tokens * (a.n_heads + 2 * a.kv.n_kv_heads) * (a.kv.head_dim / 2);
-  const size_t blocks = (total + 255) / 256;
-  k_rope_append_paged<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(a);
-  return cudaGetLastError();
+  const uint32_t size = a.dtype == NRC_F32 ? 4 : 2;
+  // Every bit below the access width is 0 in what all accesses start from (the pages' strides are checked already).
+  uint64_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                 reinterpret_cast<uintptr_t>(a.q_out);
+  for (int64_t stride : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head, a.qo_token, a.qo_head})
+    low |= (uint64_t)stride * size;
+  if (a.style == 1) low |= (uint64_t)(a.rot_dim / 2) * size;
+  uint32_t w = 16 / size;
+  while (w > 1 && low % (w * size)) w /= 2;
+  return a.dtype == NRC_F32   ? launch_rope_w<NRC_F32>(a, w, s)
+         : a.dtype == NRC_F16 ? launch_rope_w<NRC_F16>(a, w, s)
+                              : launch_rope_w<NRC_BF16>(a, w, s);
 }
 
 cudaError_t kv_evict_run(const EvictArgs& a, cudaStream_t s) {
   k_evict_select<<<dim3(a.kv.n_kv_heads, a.kv.n_seqs), EV_THREADS, 0, s>>>(a);
   if (cudaError_t e = cudaGetLastError()) return e;
-  k_evict_move<<<dim3(a.kv.n_kv_heads, a.kv.n_seqs, 2), EV_THREADS, 0, s>>>(a);
-  return cudaGetLastError();
+  // Columns of at least 32 bytes, until some two blocks per SM share the rows.
+  uint32_t pieces = a.kv.head_dim / 8, cols = 1;
+  while (pieces % 2 == 0 && pieces > 2 && (uint64_t)a.kv.n_kv_heads * a.kv.n_seqs * 2 * cols < 296) pieces /= 2, cols *= 2;
+  EvictArgs aa = a;
+  void* args[] = {&aa, &pieces};
+  return launch_kernel((const void*)k_evict_move, dim3(a.kv.n_kv_heads * cols, a.kv.n_seqs, 2), dim3(MV_THREADS), 0, s, true,
+                       args);
 }
 
 cudaError_t paged_take_errors(unsigned* bits) {
