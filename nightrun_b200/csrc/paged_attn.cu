@@ -15,22 +15,30 @@ int sm_count() {
   return n;
 }
 
+// Parts of the cache's type that hold the bits of q's (and out's) type.
+int parts_of(int cache, int dtype) {
+  if (cache == NRC_F16) return dtype == NRC_F32 ? 2 : 1;
+  return dtype == NRC_F32 ? 3 : dtype == NRC_F16 ? 2 : 1;
+}
+
 // Fills the plan and returns the workspace's bytes; `base` null: sizes only.
 size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   const nrc_paged_kv& kv = p.a.kv;
   p.gqa = p.a.n_heads / kv.n_kv_heads;
   p.rows = p.gqa * p.a.n_new;
-  *nt = p.rows <= 8 ? 1 : p.rows <= 16 || kv.head_dim > pattn::MAX_HD_NT4 ? 2 : 4;
+  *nt = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
   const uint32_t cols = 8 * *nt;
   p.row_blocks = (p.rows + cols - 1) / cols;
   const uint64_t items = (uint64_t)kv.n_seqs * kv.n_kv_heads * p.row_blocks;
   const uint32_t units = (p.a.max_len + pattn::UNIT - 1) / pattn::UNIT;
+  p.step_pages = pattn::UNIT / kv.page_size;
+  p.step_off = pattn::UNIT % kv.page_size;
   p.min_units = 4;
   p.direct = units <= p.min_units && items <= 0x7fffffffu;
   if (p.direct) {
     p.blocks = (uint32_t)items;
   } else {
-    const uint64_t all = items * units, resident = (uint64_t)sm_count() * (*nt == 1 ? 3 : 2);
+    const uint64_t all = items * units, resident = (uint64_t)sm_count() * pattn::resident(kv.head_dim, *nt);
     const uint64_t want = (all + p.min_units - 1) / p.min_units;
     p.blocks = (uint32_t)(want < resident ? want : resident);
   }
@@ -42,7 +50,7 @@ size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   };
   if (!p.direct) {
     p.cut = reinterpret_cast<int4*>(take(sizeof(int4) * p.blocks));
-    p.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * 2 * p.blocks * cols));
+    p.part_nl = reinterpret_cast<float2*>(take(sizeof(float2) * 2 * p.blocks * cols));
     p.part_o = reinterpret_cast<float*>(take(sizeof(float) * 2 * p.blocks * cols * kv.head_dim));
   }
   p.lse = nullptr;
@@ -71,11 +79,9 @@ cudaError_t paged_attn_run(const PagedAttnArgs& a, cudaStream_t s) {
   void* err = nullptr;
   if (cudaError_t e = cudaGetSymbolAddress(&err, g_attn_err)) return e;
   p.err = static_cast<unsigned*>(err);
-  // Parts of the cache's type that hold the bits of q's (and out's) type.
-  if (a.kv.dtype == NRC_F16) return a.dtype == NRC_F32 ? paged_attn_f16_2(p, nt, s) : paged_attn_f16_1(p, nt, s);
-  return a.dtype == NRC_F32   ? paged_attn_bf16_3(p, nt, s)
-         : a.dtype == NRC_F16 ? paged_attn_bf16_2(p, nt, s)
-                              : paged_attn_bf16_1(p, nt, s);
+  const int parts = parts_of(a.kv.dtype, a.dtype);
+  if (a.kv.dtype == NRC_F16) return parts == 2 ? paged_attn_f16_2(p, nt, s) : paged_attn_f16_1(p, nt, s);
+  return parts == 3 ? paged_attn_bf16_3(p, nt, s) : parts == 2 ? paged_attn_bf16_2(p, nt, s) : paged_attn_bf16_1(p, nt, s);
 }
 
 cudaError_t paged_attn_take_errors(unsigned* bits) {

@@ -13,17 +13,19 @@
 //
 // Layout. Both products run transposed, with the cache as the 16-row operand A of mma.m16n8k16 and the query rows as
 // its 8 columns: S^T = K Q^T (16 positions x 8 rows) and O^T += V^T P^T (16 values x 8 rows), so that 1..8 rows waste
-// nothing more than their tile. The order of the contracted index is free, and A's fragment can be loaded straight
-// from global memory in 16-byte pieces:
-//   K: lane (g, t) = (lane / 4, lane % 4) reads the values 32 c + 8 t .. + 7 of the positions g and g + 8: two k-steps
+// nothing more than their tile. The order of the contracted index is free, so a lane's share of an operand can be
+// whole 16-byte pieces of cached rows:
+//   K: lane (g, t) = (lane / 4, lane % 4) holds the values 32 c + 8 t .. + 7 of the positions g and g + 8: two k-steps
 //      of A, whose k index 2 t + {0, 1} stands for value 32 c + 8 t + 4 s + {0, 1} and 2 t + 8 + {0, 1} for the two
 //      behind them. Q's fragment in shared memory is laid out for the same order.
-//   V: lane (g, t) reads the values 64 c + 8 g .. + 7 of the positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9; byte permutes
+//   V: lane (g, t) holds the values 64 c + 8 g .. + 7 of the positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9; byte permutes
 //      pair neighbouring positions, and row g of the tile j of chunk c stands for value 64 c + 8 g + 2 j, row g + 8 for
 //      the one behind it.
-// P^T's operand is the transposed accumulator of S^T, turned by movmatrix. No tile passes through shared memory, and a
-// warp has 16 positions of K and V in flight while it computes on the ones before. tcgen05 would need the tiles in
-// shared memory and 64 or more rows of queries to be fed; here its rate is not what is missing.
+// P^T's operand is the transposed accumulator of S^T, turned by movmatrix. No tile passes through shared memory: the
+// pieces of the next tile are loaded into the registers of the one before as soon as those are used, 8 KB (of
+// 128-wide f16 heads) per warp in flight. (Pieces copied ahead into shared memory, 190 KB per SM in flight, were
+// slower: 248 against 199 us for 983 MB. It is the warps' instructions per tile that count, not the bytes in
+// flight.) tcgen05 would need 64 or more rows of queries to be fed; its rate is not what is missing.
 //
 // Split parts. The tensor cores take operands of the cache's type. q (scaled by a power of two to at most 2 per row) and
 // p enter as PARTS values of that type whose sum holds the bits that the output's type can show: one where the output is
@@ -38,7 +40,8 @@ namespace pattn {
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int TILE = 16;             // positions per warp and step
 constexpr int UNIT = TILE * WARPS;   // positions per block and step: the unit of the schedule
-constexpr int MAX_HD_NT4 = 64;       // 32 query rows at once: wider heads' accumulators do not fit the registers
+// Blocks per SM, by the registers.
+constexpr int resident(int hd, int nt) { return nt > 1 ? 2 : hd <= 32 ? 4 : 3; }
 
 // What one launch needs beside the arguments.
 struct Plan {
@@ -49,8 +52,9 @@ struct Plan {
   uint32_t min_units;
   int4* cut;                       // [blocks]: the work that starts in this block and ends in a later one
   float* lse;                      // [n_seqs][n_heads * n_new] (row order), for the weights
-  float2* part_ml;                 // [2 * blocks][8 * NT]
+  float2* part_nl;                 // [2 * blocks][8 * NT]: reference and sum
   float* part_o;                   // [2 * blocks][8 * NT][head_dim]
+  uint32_t step_pages, step_off;   // UNIT positions in pages and the rest
   unsigned* err;
 };
 
@@ -103,12 +107,12 @@ NRC_DEV void split2(float x, float y, uint32_t (&out)[PARTS]) {
   }
 }
 
-NRC_DEV uint4 ld_stream16(const void* p) {
+NRC_DEV uint4 ldg16(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-NRC_DEV uint2 ld_stream8(const void* p) {
+NRC_DEV uint2 ldg8(const void* p) {
   uint2 v;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
@@ -127,74 +131,134 @@ NRC_DEV uint32_t seq_len(const Plan& p, uint32_t b) {
 // Units of a sequence; an empty one has a unit too, whose block writes its zeros.
 NRC_DEV uint32_t units_of(uint32_t len) { return len ? (len + UNIT - 1) / UNIT : 1u; }
 
-// The positions of one tile: element offset of each lane's position (lane & 15), and which of the 16 can be read.
-struct TileRows {
-  int64_t off;
-  uint32_t ok;  // bit r: position r of the tile is cached
+// K pieces of a tile: [chunk of 32 values][position g or g + 8].
+template <int HD>
+struct KTile {
+  uint4 w[HD / 32][2];
 };
-NRC_DEV TileRows tile_rows(const Plan& p, uint32_t b, int64_t head_off, uint32_t tile, uint32_t len, int lane) {
-  const uint32_t pos = tile * TILE + (lane & 15);
-  TileRows t;
-  t.off = -1;
-  if (pos < len) {
-    t.off = paged_row(p.a.kv, b, pos);
-    if (t.off < 0)
-      atomicOr(p.err, ERR_BAD_PAGE);
-    else
-      t.off += head_off;
-  }
-  t.ok = __ballot_sync(0xffffffffu, t.off >= 0) & 0xffffu;
-  return t;
-}
-
+// V pieces of a tile: whole chunks of 64 values (16 bytes per position), a last chunk of 32 (8 bytes).
 template <int HD>
-NRC_DEV void load_k(uint4 (&k)[HD / 32][2], const uint16_t* base, const TileRows& r, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int64_t off = __shfl_sync(0xffffffffu, r.off, g + 8 * i);
-    const uint16_t* p = base + off + 8 * t;
-#pragma unroll
-    for (int c = 0; c < HD / 32; c++) k[c][i] = off >= 0 ? ld_stream16(p + 32 * c) : make_uint4(0, 0, 0, 0);
-  }
-}
-
-// V: whole chunks of 64 values as 16-byte pieces, a last chunk of 32 as 8-byte pieces.
-template <int HD>
-struct VRegs {
+struct VTile {
   uint4 w[HD / 64 > 0 ? HD / 64 : 1][4];
   uint2 h[4];
-};
-template <int HD>
-NRC_DEV void load_v(VRegs<HD>& v, const uint16_t* base, const TileRows& r, int lane) {
-  const int g = lane >> 2, t = lane & 3;
+  // Operand A of value tile mt: rows g, g + 8 (two neighbouring values), k = positions.
+  NRC_DEV void operand(uint32_t (&a)[4], int mt) const {
+    uint32_t x[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int64_t off = __shfl_sync(0xffffffffu, r.off, 2 * t + (i & 1) + 8 * (i >> 1));
-    const uint16_t* p = base + off;
-#pragma unroll
-    for (int c = 0; c < HD / 64; c++) v.w[c][i] = off >= 0 ? ld_stream16(p + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
-    if (HD % 64) v.h[i] = off >= 0 ? ld_stream8(p + HD - 32 + 4 * g) : make_uint2(0, 0);
+    for (int i = 0; i < 4; i++) {
+      if (mt < HD / 64 * 4) {
+        const uint4& q = w[mt / 4][i];
+        x[i] = mt % 4 == 0 ? q.x : mt % 4 == 1 ? q.y : mt % 4 == 2 ? q.z : q.w;
+      } else {
+        x[i] = mt % 2 == 0 ? h[i].x : h[i].y;
+      }
+    }
+    a[0] = __byte_perm(x[0], x[1], 0x5410);
+    a[1] = __byte_perm(x[0], x[1], 0x7632);
+    a[2] = __byte_perm(x[2], x[3], 0x5410);
+    a[3] = __byte_perm(x[2], x[3], 0x7632);
   }
-}
-// Operand A of value tile mt: rows g, g + 8 (two neighbouring values), k = positions.
-template <int HD>
-NRC_DEV void v_operand(uint32_t (&a)[4], const VRegs<HD>& v, int mt) {
-  uint32_t x[4];
+};
+
+// A warp's way through its tiles, every WARPS-th from `tile` on below position `end`. Where pages are whole tiles
+// (page_size % 16 == 0) one lookup, alike in all lanes, serves a tile; else each lane looks its position up.
+struct Walk {
+  const uint8_t *k, *v;    // the KV head's row 0 (in bytes), this lane's piece
+  const int32_t* table;
+  int64_t row;             // byte offset of the current tile's first row (or of this lane's), -1: none
+  int64_t step;            // bytes between positions
+  uint32_t end, pos;       // pos: of the tile looked up next (its first, or this lane's own)
+  uint32_t pi, off;        // page index and offset of pos
+  int32_t page;            // table[pi], read one tile ahead
+  uint32_t left;           // positions of the current tile before the end
+  bool in_page;
+  bool bad;                // a page outside the pool was met: tiles have to be masked by cached()
+
+  NRC_DEV void fetch() { page = pos < end ? table[pi] : 0; }
+  NRC_DEV void begin(const Plan& p, uint32_t b, uint32_t h, uint32_t tile, uint32_t end_, int lane) {
+    k = static_cast<const uint8_t*>(p.a.kv.k) + (int64_t)h * p.a.kv.head_stride * 2 + 16 * (lane & 3);
+    v = static_cast<const uint8_t*>(p.a.kv.v) + (int64_t)h * p.a.kv.head_stride * 2;
+    table = p.a.kv.table + (size_t)b * p.a.kv.table_stride;
+    step = p.a.kv.pos_stride * 2;
+    end = end_;
+    in_page = p.a.kv.page_size % TILE == 0;
+    bad = false;
+    pos = tile * TILE + (in_page ? 0 : lane & 15);
+    pi = pos / p.a.kv.page_size;
+    off = pos - pi * p.a.kv.page_size;
+    fetch();
+  }
+  // Makes the tile at `pos` the current one and moves on.
+  NRC_DEV void next(const Plan& p, int lane) {
+    const uint32_t tile0 = in_page ? pos : pos - (lane & 15);
+    left = tile0 < end ? min(end - tile0, (uint32_t)TILE) : 0;
+    const bool live = pos < end, found = (uint32_t)page < p.a.kv.n_pages;
+    row = live && found ? ((int64_t)page * p.a.kv.page_stride + (int64_t)off * p.a.kv.pos_stride) * 2 : -1;
+    if (__any_sync(0xffffffffu, live && !found)) {
+      if (live && !found) atomicOr(p.err, ERR_BAD_PAGE);
+      bad = true;
+    }
+    pos += UNIT;
+    pi += p.step_pages;
+    off += p.step_off;
+    if (off >= p.a.kv.page_size) {
+      off -= p.a.kv.page_size;
+      pi++;
+    }
+    fetch();
+  }
+  // All 16 rows can be read at row + r * step.
+  NRC_DEV bool plain() const { return in_page && left == TILE && row >= 0; }
+  NRC_DEV int64_t row_of(int r) const {
+    if (in_page) return row >= 0 && (uint32_t)r < left ? row + r * step : -1;
+    return __shfl_sync(0xffffffffu, row, r);
+  }
+  template <int HD>
+  NRC_DEV void load_k(KTile<HD>& t, int lane) const {
+    const int g = lane >> 2;
+    if (plain()) {
+      const uint8_t* p0 = k + (row + g * step);
+      const uint8_t* p1 = p0 + 8 * step;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (mt < HD / 64 * 4) {
-      const uint4& w = v.w[mt / 4][i];
-      x[i] = mt % 4 == 0 ? w.x : mt % 4 == 1 ? w.y : mt % 4 == 2 ? w.z : w.w;
-    } else {
-      x[i] = mt % 2 == 0 ? v.h[i].x : v.h[i].y;
+      for (int c = 0; c < HD / 32; c++) t.w[c][0] = ldg16(p0 + 64 * c), t.w[c][1] = ldg16(p1 + 64 * c);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int64_t o = row_of(g + 8 * i);
+#pragma unroll
+      for (int c = 0; c < HD / 32; c++) t.w[c][i] = o >= 0 ? ldg16(k + o + 64 * c) : make_uint4(0, 0, 0, 0);
     }
   }
-  a[0] = __byte_perm(x[0], x[1], 0x5410);
-  a[1] = __byte_perm(x[0], x[1], 0x7632);
-  a[2] = __byte_perm(x[2], x[3], 0x5410);
-  a[3] = __byte_perm(x[2], x[3], 0x7632);
-}
+  template <int HD>
+  NRC_DEV void load_v(VTile<HD>& t, int lane) const {
+    const int g = lane >> 2, q = lane & 3;
+    if (plain()) {
+      const uint8_t* p0 = v + (row + 2 * q * step);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint8_t* pr = p0 + ((i & 1) + 8 * (i >> 1)) * step;
+#pragma unroll
+        for (int c = 0; c < HD / 64; c++) t.w[c][i] = ldg16(pr + 16 * g + 128 * c);
+        if (HD % 64) t.h[i] = ldg8(pr + 8 * g + 2 * (HD - 32));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t o = row_of(2 * q + (i & 1) + 8 * (i >> 1));
+#pragma unroll
+      for (int c = 0; c < HD / 64; c++) t.w[c][i] = o >= 0 ? ldg16(v + o + 16 * g + 128 * c) : make_uint4(0, 0, 0, 0);
+      if (HD % 64) t.h[i] = o >= 0 ? ldg8(v + o + 8 * g + 2 * (HD - 32)) : make_uint2(0, 0);
+    }
+  }
+  // Which positions of a tile are cached, where a bad page was met.
+  NRC_DEV uint32_t cached(const Plan& p, uint32_t b, uint32_t p0, int lane) const {
+    const uint32_t at = p0 + (lane & 15);
+    return __ballot_sync(0xffffffffu, at < end && paged_row(p.a.kv, b, at) >= 0) & 0xffffu;
+  }
+};
+
 // The first of the two neighbouring values that rows g and g + 8 of tile mt stand for.
 template <int HD>
 NRC_DEV int value_of(int mt, int g) {
@@ -240,38 +304,47 @@ NRC_DEV void load_queries(const Plan& p, uint32_t b, uint32_t h, uint32_t rb, Qu
   if (part == 0) qs.factor[row] = ldexpf(p.a.scale * 1.44269504088896340736f, e);
 }
 
-// S^T of one tile.
+// S^T of a tile. Few columns: two chains of products, so that one's latency hides the other's.
 template <bool BF, int HD, int PARTS, int NT>
-NRC_DEV void scores(float (&s)[NT][4], const uint4 (&k)[HD / 32][2], const Queries<HD, PARTS, NT>& qs, int lane) {
+NRC_DEV void scores(float (&s)[NT][4], const KTile<HD>& k, const Queries<HD, PARTS, NT>& qs, int lane) {
+  constexpr int CHAINS = NT == 1 ? 2 : 1;
+  float x[CHAINS][NT][4];
+#pragma unroll
+  for (int u = 0; u < CHAINS; u++)
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[u][n][i] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < HD / 32; c++) {
+    const uint4 k0 = k.w[c][0], k1 = k.w[c][1];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint32_t a[4] = {u ? k0.z : k0.x, u ? k1.z : k1.x, u ? k0.w : k0.y, u ? k1.w : k1.y};
+#pragma unroll
+      for (int j = 0; j < PARTS; j++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const uint2 q = qs.frag[j][2 * c + u][n][lane];
+          mma<BF>(x[u % CHAINS][n], a, q.x, q.y);
+        }
+    }
+  }
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) s[n][i] = 0.0f;
-#pragma unroll
-  for (int c = 0; c < HD / 32; c++)
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const uint32_t a[4] = {u ? k[c][0].z : k[c][0].x, u ? k[c][1].z : k[c][1].x, u ? k[c][0].w : k[c][0].y,
-                             u ? k[c][1].w : k[c][1].y};
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int j = 0; j < PARTS; j++) {
-          const uint2 q = qs.frag[j][2 * c + u][n][lane];
-          mma<BF>(s[n], a, q.x, q.y);
-        }
-    }
+    for (int i = 0; i < 4; i++) s[n][i] = CHAINS == 2 ? x[0][n][i] + x[CHAINS - 1][n][i] : x[0][n][i];
 }
 
 // Where block `i` starts, and the units each block takes: sequences in order, in each the (KV head, row
-// block) pairs in order, in each its units. Every block finds its start alone, from the lengths.
+// block) pairs in order (hbs of them), in each its units. Every block finds its start alone, from the lengths.
 struct Start {
-  uint32_t b, hb, unit;  // sequence, KV head * row_blocks + row block, first unit
+  uint32_t b, hb, unit;  // sequence, pair, first unit
   uint64_t left;         // units of work of this block
   uint64_t share, total;
 };
-NRC_DEV Start find_start(const Plan& p, uint64_t* warp_sums, Start* found) {
-  const uint32_t hbs = p.a.kv.n_kv_heads * p.row_blocks, n = p.a.kv.n_seqs;
+NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start* found) {
+  const uint32_t n = p.a.kv.n_seqs;
   const uint32_t per = (n + THREADS - 1) / THREADS, b0 = min(threadIdx.x * per, n), b1 = min(b0 + per, n);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t sum = 0;
@@ -311,18 +384,23 @@ NRC_DEV Start find_start(const Plan& p, uint64_t* warp_sums, Start* found) {
   return *found;
 }
 
+// A score's exponential is taken as 2^(s + ref): ref is LIFT less the largest score seen when the row's reference was last
+// set, and is set again (its sums rescaled) when an exponent passes LIFT + SLACK, so most tiles need no reduction over
+// their positions. f16 weights: up to 2^15, and with bits down to 2^-24, 2^-32 of the row's sum. UNSET: nothing seen.
+constexpr float SLACK = 7.0f, LIFT = 8.0f, UNSET = 3e38f;
+
 template <bool BF, int HD, int PARTS, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p) {
+__global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid_constant__ Plan p) {
   constexpr int MT = HD / 16, COLS = 8 * NT;
-  // A running sum of p, whose f16 operand has no bits below 2^-24: p is kept 2^14 times larger.
-  constexpr float LIFT = BF ? 0.0f : 14.0f;
+  extern __shared__ __align__(16) uint8_t dyn_s[];  // the warps' sums, to be joined
   __shared__ Queries<HD, PARTS, NT> qs;
-  __shared__ __align__(16) float o_s[WARPS][COLS][HD + 2];
-  __shared__ float m_s[WARPS][COLS], l_s[WARPS][COLS];
+  __shared__ float n_s[WARPS][COLS], l_s[WARPS][COLS];
   __shared__ uint64_t warp_sums[WARPS];
   __shared__ Start start_s;
+  float(*o_s)[COLS][HD + 2] = reinterpret_cast<float(*)[COLS][HD + 2]>(dyn_s);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t hbs = p.a.kv.n_kv_heads * p.row_blocks;
+  pdl_trigger();  // the join waits for this grid's end by itself
   Start st;
   if (p.direct) {
     st.b = blockIdx.x / hbs;
@@ -331,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
     st.left = units_of(seq_len(p, st.b));
     st.share = st.left;
   } else {
-    st = find_start(p, warp_sums, &start_s);
+    st = find_start(p, hbs, warp_sums, &start_s);
     if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   bool first = true;
@@ -340,22 +418,23 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
     const uint32_t len = seq_len(p, b), units = units_of(len), u0 = st.unit;
     const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + st.left);
     __syncthreads();  // the queries and sums of the work before are read
+    const uint32_t end = min(u1 * UNIT, len);
+    Walk walk;
+    walk.begin(p, b, h, u0 * WARPS + warp, end, lane);
+    KTile<HD> k;
+    VTile<HD> v;
+    walk.next(p, lane);
+    walk.load_k<HD>(k, lane);
+    walk.load_v<HD>(v, lane);
     load_queries<BF, HD, PARTS, NT>(p, b, h, rb, qs);
     __syncthreads();
-    const uint16_t* kb = static_cast<const uint16_t*>(p.a.kv.k);
-    const uint16_t* vb = static_cast<const uint16_t*>(p.a.kv.v);
-    const int64_t head_off = (int64_t)h * p.a.kv.head_stride;
-    float acc[MT][NT][4], m[NT][2], l[NT][2], fac[NT][2];
-    uint32_t sees[NT][2];
+    float acc[MT][NT][4], ref[NT][2], l[NT][2], fac[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const uint32_t r = rb * COLS + 8 * n + 2 * t + i;
-        const uint32_t behind = r < p.rows ? p.a.n_new - 1 - r / p.gqa : 0;
-        sees[n][i] = len > behind ? len - behind : 0;
         fac[n][i] = qs.factor[8 * n + 2 * t + i];
-        m[n][i] = -INFINITY;
+        ref[n][i] = UNSET;
         l[n][i] = 0.0f;
       }
 #pragma unroll
@@ -365,52 +444,54 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[j][n][i] = 0.0f;
     const uint32_t all_see = len > p.a.n_new - 1 ? len - (p.a.n_new - 1) : 0;  // every row sees these
+    // Positions that column c of this lane's tiles sees.
+    auto sees = [&](int c) -> uint32_t {
+      const uint32_t r = rb * COLS + c, behind = r < p.rows ? p.a.n_new - 1 - r / p.gqa : 0;
+      return len > behind ? len - behind : 0;
+    };
 
-    uint4 k[HD / 32][2];
-    VRegs<HD> v;
-    const uint32_t tiles = min(u1 * WARPS, (len + TILE - 1) / TILE);
-    uint32_t tile = u0 * WARPS + warp;
-    TileRows now = tile_rows(p, b, head_off, tile, tile < tiles ? len : 0, lane);
-    load_k<HD>(k, kb, now, lane);
-    load_v<HD>(v, vb, now, lane);
-    TileRows next = tile_rows(p, b, head_off, tile + WARPS, tile + WARPS < tiles ? len : 0, lane);
-    for (; tile < tiles; tile += WARPS) {
-      float s[NT][4];
+    for (uint32_t p0 = (u0 * WARPS + warp) * TILE; p0 < end; p0 += UNIT) {
+      float s[NT][4], e[NT][4];
       scores<BF, HD, PARTS, NT>(s, k, qs, lane);
-      load_k<HD>(k, kb, next, lane);
-      const uint32_t p0 = tile * TILE;
-      const bool whole = now.ok == 0xffffu && p0 + TILE <= all_see;
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          s[n][i] *= fac[n][i & 1];
-          const uint32_t r = g + 8 * (i >> 1);
-          if (!whole && (!((now.ok >> r) & 1) || p0 + r >= sees[n][i & 1])) s[n][i] = -INFINITY;
-        }
-      float top[NT][2];
+      walk.next(p, lane);
+      walk.load_k<HD>(k, lane);
+      const bool whole = p0 + TILE <= all_see && !walk.bad;
       bool grows = false;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          float x = fmaxf(s[n][i], s[n][i + 2]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          top[n][i] = x;
-          grows = grows || x > m[n][i];
-        }
+        for (int i = 0; i < 4; i++) e[n][i] = fmaf(s[n][i], fac[n][i & 1], ref[n][i & 1]);
+      if (!whole) {
+        const uint32_t ok = walk.bad ? walk.cached(p, b, p0, lane) : 0xffffu;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t r = g + 8 * (i >> 1);
+            if (!((ok >> r) & 1) || p0 + r >= sees(8 * n + 2 * t + (i & 1))) e[n][i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        grows = grows || fmaxf(fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3])) > LIFT + SLACK;
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float f[2];
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float mn = fmaxf(m[n][i], top[n][i]);
-            f[i] = m[n][i] == -INFINITY ? 0.0f : exp2_fast(m[n][i] - mn);
-            m[n][i] = mn;
+            const float x0 = e[n][i] == -INFINITY ? -INFINITY : s[n][i] * fac[n][i];
+            const float x1 = e[n][i + 2] == -INFINITY ? -INFINITY : s[n][i + 2] * fac[n][i];
+            float x = fmaxf(x0, x1);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float now = fminf(ref[n][i], LIFT - x);
+            f[i] = exp2_fast(now - ref[n][i]);
+            ref[n][i] = now;
             l[n][i] *= f[i];
+            e[n][i] = x0 + now;
+            e[n][i + 2] = x1 + now;
           }
 #pragma unroll
           for (int j = 0; j < MT; j++)
@@ -421,17 +502,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
       uint32_t pb[NT][PARTS][2];
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float e[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          // A row that has seen nothing yet: its scores are all -inf, any finite maximum gives 0.
-          const float ref = m[n][i & 1] == -INFINITY ? 0.0f : m[n][i & 1] - LIFT;
-          e[i] = exp2_fast(s[n][i] - ref);
-          l[n][i & 1] += e[i];
+          e[n][i] = exp2_fast(e[n][i]);
+          l[n][i & 1] += e[n][i];
         }
         uint32_t lo[PARTS], hi[PARTS];
-        split2<BF, PARTS>(e[0], e[1], lo);
-        split2<BF, PARTS>(e[2], e[3], hi);
+        split2<BF, PARTS>(e[n][0], e[n][1], lo);
+        split2<BF, PARTS>(e[n][2], e[n][3], hi);
 #pragma unroll
         for (int j = 0; j < PARTS; j++) {
           pb[n][j][0] = transpose8x8(lo[j]);
@@ -442,25 +520,25 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
 #pragma unroll
         for (int j = 0; j < MT; j++) {
           uint32_t a[4];
-          v_operand<HD>(a, v, j);
+          v.operand(a, j);
 #pragma unroll
-          for (int n = 0; n < NT; n++)
+          for (int i = 0; i < PARTS; i++)
 #pragma unroll
-            for (int i = 0; i < PARTS; i++) mma<BF>(acc[j][n], a, pb[n][i][0], pb[n][i][1]);
+            for (int n = 0; n < NT; n++) mma<BF>(acc[j][n], a, pb[n][i][0], pb[n][i][1]);
         }
       } else {
         // Positions that only some of the new tokens see: 0 times an infinite value must not reach the others, so
         // each token's rows are taken from a product with the values behind it cleared.
         const uint32_t tok0 = rb * COLS / p.gqa, tok1 = min(p.a.n_new, (rb * COLS + COLS - 1) / p.gqa + 1);
         for (uint32_t tok = tok0; tok < tok1; tok++) {
-          const uint32_t behind = p.a.n_new - 1 - tok, end = len > behind ? len - behind : 0;
+          const uint32_t behind = p.a.n_new - 1 - tok, stop = len > behind ? len - behind : 0;
           const uint32_t at = p0 + 2 * t;
-          const uint32_t mask0 = (at < end ? 0xffffu : 0u) | (at + 1 < end ? 0xffff0000u : 0u);
-          const uint32_t mask1 = (at + 8 < end ? 0xffffu : 0u) | (at + 9 < end ? 0xffff0000u : 0u);
+          const uint32_t mask0 = (at < stop ? 0xffffu : 0u) | (at + 1 < stop ? 0xffff0000u : 0u);
+          const uint32_t mask1 = (at + 8 < stop ? 0xffffu : 0u) | (at + 9 < stop ? 0xffff0000u : 0u);
 #pragma unroll
           for (int j = 0; j < MT; j++) {
             uint32_t a[4];
-            v_operand<HD>(a, v, j);
+            v.operand(a, j);
             a[0] &= mask0, a[1] &= mask0, a[2] &= mask1, a[3] &= mask1;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -474,9 +552,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
           }
         }
       }
-      load_v<HD>(v, vb, next, lane);
-      now = next;
-      next = tile_rows(p, b, head_off, tile + 2 * WARPS, tile + 2 * WARPS < tiles ? len : 0, lane);
+      walk.load_v<HD>(v, lane);
     }
 
     // Join the warps.
@@ -487,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], o);
         if (g == 0) {
-          m_s[warp][8 * n + 2 * t + i] = m[n][i];
+          n_s[warp][8 * n + 2 * t + i] = ref[n][i];
           l_s[warp][8 * n + 2 * t + i] = l[n][i];
         }
       }
@@ -501,30 +577,30 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
     }
     __syncthreads();
     const bool complete = u0 == 0 && u1 == units;
-    const uint32_t slot = 2 * blockIdx.x + (first && u0 ? 0 : 1);
+    const uint32_t part = 2 * blockIdx.x + (first && u0 ? 0 : 1);
     for (uint32_t i = threadIdx.x; i < COLS * HD; i += THREADS) {
       const uint32_t col = i / HD, d = i % HD, r = rb * COLS + col;
       if (r >= p.rows) break;
-      float mx = -INFINITY, o = 0.0f, sum = 0.0f;
+      float low = n_s[0][col], o = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, m_s[w][col]);
+      for (int w = 1; w < WARPS; w++) low = fminf(low, n_s[w][col]);
 #pragma unroll
       for (int w = 0; w < WARPS; w++) {
-        const float f = m_s[w][col] == -INFINITY ? 0.0f : exp2_fast(m_s[w][col] - mx);
+        const float f = exp2_fast(low - n_s[w][col]);
         sum += f * l_s[w][col];
         o += f * o_s[w][col][d];
       }
       if (complete) {
         const uint32_t tok = r / p.gqa, head = h * p.gqa + r % p.gqa;
         store_from_f32(p.a.out, (int64_t)b * p.a.o_seq + (int64_t)tok * p.a.o_token + (int64_t)head * p.a.o_head + d,
-                       p.a.dtype, mx == -INFINITY ? 0.0f : o / sum);
-        if (d == 0 && p.lse) p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = mx - LIFT + log2f(sum);
+                       p.a.dtype, sum == 0.0f ? 0.0f : o / sum);
+        if (d == 0 && p.lse) p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = log2f(sum) - low;
       } else {
-        p.part_o[((size_t)slot * COLS + col) * HD + d] = o;
-        if (d == 0) p.part_ml[(size_t)slot * COLS + col] = make_float2(mx, sum);
+        p.part_o[((size_t)part * COLS + col) * HD + d] = o;
+        if (d == 0) p.part_nl[(size_t)part * COLS + col] = make_float2(low, sum);
       }
     }
-    // Work that starts here and goes on: the join kernel's item, with the blocks that hold its parts.
+    // Work that starts here and goes on: the join kernel's item, with the number of blocks that hold its parts.
     if (u1 < units && !(first && u0) && threadIdx.x == 0) {
       const uint64_t rest = units - u1;
       p.cut[blockIdx.x] = make_int4((int)b, (int)st.hb, (int)(1 + (rest + st.share - 1) / st.share), 0);
@@ -537,119 +613,146 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) k_attn(const Plan p)
       st.b++;
     }
   }
-  pdl_trigger();
 }
 
-// One block per (attention block whose last work goes on, row): the parts' running maxima and sums joined.
+// One block per (attention block whose last work goes on, row): the parts' references and sums joined, the parts dealt
+// to JOIN_THREADS / HD groups of threads.
+constexpr int JOIN_THREADS = 384;
 template <int HD>
-__global__ void __launch_bounds__(HD) k_join(const Plan p, int cols, float lift) {
+__global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ Plan p, int cols) {
+  constexpr int GROUPS = JOIN_THREADS / HD;
+  __shared__ float o_s[GROUPS][HD], l_s[GROUPS];
+  pdl_trigger();
   pdl_wait();
   const int4 cut = p.cut[blockIdx.x];
   const uint32_t b = cut.x, h = cut.y / p.row_blocks, rb = cut.y % p.row_blocks, n = cut.z;
-  const uint32_t col = blockIdx.y, r = rb * cols + col;
+  const uint32_t col = blockIdx.y, r = rb * cols + col, d = threadIdx.x % HD, group = threadIdx.x / HD;
   if (n == 0 || r >= p.rows) return;
   // The first part is the last work of its block, the others the first of theirs.
-  auto slot = [&](uint32_t i) { return ((size_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * cols + col; };
-  float mx = -INFINITY;
-  for (uint32_t i = 0; i < n; i++) mx = fmaxf(mx, p.part_ml[slot(i)].x);
+  auto part = [&](uint32_t i) { return ((size_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * cols + col; };
+  float low = UNSET;
+  for (uint32_t i = threadIdx.x & 31; i < n; i += 32) low = fminf(low, p.part_nl[part(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   float o = 0.0f, sum = 0.0f;
-#pragma unroll 4
-  for (uint32_t i = 0; i < n; i++) {
-    const float2 ml = p.part_ml[slot(i)];
-    const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mx);
-    sum += f * ml.y;
-    o += f * p.part_o[slot(i) * HD + threadIdx.x];
+#pragma unroll 8
+  for (uint32_t i = group; i < n; i += GROUPS) {
+    const float2 nl = p.part_nl[part(i)];
+    const float f = exp2_fast(low - nl.x);
+    sum += f * nl.y;
+    o += f * p.part_o[part(i) * HD + d];
   }
+  o_s[group][d] = o;
+  if (d == 0) l_s[group] = sum;
+  __syncthreads();
+  if (group) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; i++) o += o_s[i][d], sum += l_s[i];
   const uint32_t tok = r / p.gqa, head = h * p.gqa + r % p.gqa;
-  store_from_f32(p.a.out, (int64_t)b * p.a.o_seq + (int64_t)tok * p.a.o_token + (int64_t)head * p.a.o_head + threadIdx.x,
-                 p.a.dtype, mx == -INFINITY ? 0.0f : o / sum);
-  if (threadIdx.x == 0 && p.lse) p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = mx - lift + log2f(sum);
+  store_from_f32(p.a.out, (int64_t)b * p.a.o_seq + (int64_t)tok * p.a.o_token + (int64_t)head * p.a.o_head + d, p.a.dtype,
+                 sum == 0.0f ? 0.0f : o / sum);
+  if (d == 0 && p.lse) p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = log2f(sum) - low;
 }
 
-// Weights: the scores again (the same products, the same bits), 2^(s - lse) summed over the query rows in
-// a fixed order and added. One warp per tile of 16 positions of a (sequence, KV head); a block's tiles are
-// the units x, x + gridDim.x, ...
+// Weights: the scores again (the same products, the same bits; they would take more memory traffic than K does), then
+// 2^(s - lse) summed over the query rows in a fixed order and added. The attention's schedule, without row blocks.
 template <bool BF, int HD, int PARTS, int NT>
-__global__ void __launch_bounds__(THREADS) k_weights(const Plan p) {
+__global__ void __launch_bounds__(THREADS) k_weights(const __grid_constant__ Plan p) {
   constexpr int COLS = 8 * NT;
   __shared__ Queries<HD, PARTS, NT> qs;
+  __shared__ uint64_t warp_sums[WARPS];
+  __shared__ Start start_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  pdl_wait();
-  const uint32_t h = blockIdx.y, b = blockIdx.z;
-  const uint32_t len = seq_len(p, b), units = (len + UNIT - 1) / UNIT;
-  const uint16_t* kb = static_cast<const uint16_t*>(p.a.kv.k);
-  float* w = p.a.weights + ((size_t)b * p.a.kv.n_kv_heads + h) * p.a.weights_len;
-  for (uint32_t rb = 0; rb < p.row_blocks; rb++) {
-    if (blockIdx.x >= units) return;
-    __syncthreads();
-    load_queries<BF, HD, PARTS, NT>(p, b, h, rb, qs);
-    __syncthreads();
-    float fac[NT][2], lse[NT][2];
-    uint32_t sees[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const uint32_t r = rb * COLS + 8 * n + 2 * t + i;
-        const uint32_t behind = r < p.rows ? p.a.n_new - 1 - r / p.gqa : 0;
-        sees[n][i] = r < p.rows && len > behind ? len - behind : 0;
-        fac[n][i] = qs.factor[8 * n + 2 * t + i];
-        lse[n][i] = sees[n][i] ? p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] : 0.0f;
-      }
-    for (uint32_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-      const uint32_t tile = unit * WARPS + warp, p0 = tile * TILE;
-      const TileRows now = tile_rows(p, b, (int64_t)h * p.a.kv.head_stride, tile, len, lane);
-      uint4 k[HD / 32][2];
-      load_k<HD>(k, kb, now, lane);
-      float s[NT][4], sum[2] = {0.0f, 0.0f};
-      scores<BF, HD, PARTS, NT>(s, k, qs, lane);
+  const uint32_t hbs = p.a.kv.n_kv_heads;
+  Start st = find_start(p, hbs, warp_sums, &start_s);
+  bool waited = false;
+  while (st.left) {
+    const uint32_t b = st.b, h = st.hb, len = seq_len(p, b), units = units_of(len), u0 = st.unit;
+    const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + st.left), end = min(u1 * UNIT, len);
+    float* w = p.a.weights + ((size_t)b * p.a.kv.n_kv_heads + h) * p.a.weights_len;
+    const uint32_t all_see = len > p.a.n_new - 1 ? len - (p.a.n_new - 1) : 0;
+    for (uint32_t rb = 0; rb < p.row_blocks; rb++) {
+      __syncthreads();
+      Walk walk;
+      walk.begin(p, b, h, u0 * WARPS + warp, end, lane);
+      KTile<HD> k;
+      walk.next(p, lane);
+      walk.load_k<HD>(k, lane);
+      load_queries<BF, HD, PARTS, NT>(p, b, h, rb, qs);
+      __syncthreads();
+      if (!waited) pdl_wait();  // the sums below are the kernels' before
+      waited = true;
+      float fac[NT][2], lse[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t r = g + 8 * (i >> 1);
-          if (((now.ok >> r) & 1) && p0 + r < sees[n][i & 1] && lse[n][i & 1] != -INFINITY)
-            sum[i >> 1] += exp2_fast(s[n][i] * fac[n][i & 1] - lse[n][i & 1]);
+        for (int i = 0; i < 2; i++) {
+          const uint32_t r = rb * COLS + 8 * n + 2 * t + i;
+          fac[n][i] = qs.factor[8 * n + 2 * t + i];
+          // A row that is none, or saw nothing, adds nothing.
+          const float x = r < p.rows ? p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] : INFINITY;
+          lse[n][i] = x == -INFINITY ? INFINITY : x;
         }
+      for (uint32_t p0 = (u0 * WARPS + warp) * TILE; p0 < end; p0 += UNIT) {
+        float s[NT][4], sum[2] = {0.0f, 0.0f};
+        scores<BF, HD, PARTS, NT>(s, k, qs, lane);
+        walk.next(p, lane);
+        walk.load_k<HD>(k, lane);
+        const bool whole = p0 + TILE <= all_see && !walk.bad;
+        const uint32_t ok = walk.bad ? walk.cached(p, b, p0, lane) : 0xffffu;
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        const uint32_t r = g + 8 * i;
-        if (t == 0 && ((now.ok >> r) & 1)) w[p0 + r] += sum[i];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float x = fmaf(s[n][i], fac[n][i & 1], -lse[n][i & 1]);
+            if (!whole) {
+              const uint32_t q = rb * COLS + 8 * n + 2 * t + (i & 1), r = g + 8 * (i >> 1);
+              const uint32_t behind = q < p.rows ? p.a.n_new - 1 - q / p.gqa : 0;
+              if (!((ok >> r) & 1) || p0 + r + behind >= len) x = -INFINITY;
+            }
+            sum[i >> 1] += exp2_fast(x);
+          }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+          const uint32_t r = g + 8 * i;
+          if (t == 0 && p0 + r < end && ((ok >> r) & 1)) w[p0 + r] += sum[i];
+        }
       }
     }
+    st.left -= u1 - u0;
+    st.unit = 0;
+    if (++st.hb == hbs) {
+      st.hb = 0;
+      st.b++;
+    }
   }
+  if (!waited) pdl_wait();
 }
 
 template <bool BF, int HD, int PARTS, int NT>
 cudaError_t launch(Plan& p, cudaStream_t s) {
   void* args[] = {&p};
-  if (cudaError_t e = launch_kernel((const void*)k_attn<BF, HD, PARTS, NT>, dim3(p.blocks), dim3(THREADS), 0, s, false, args))
-    return e;
+  const void* attn = (const void*)k_attn<BF, HD, PARTS, NT>;
+  constexpr int sums = WARPS * 8 * NT * (HD + 2) * 4;
+  if (cudaError_t e = ensure_smem_attr(attn, sums)) return e;
+  if (cudaError_t e = launch_kernel(attn, dim3(p.blocks), dim3(THREADS), sums, s, false, args)) return e;
   if (!p.direct) {
     int cols = 8 * NT;
-    float lift = BF ? 0.0f : 14.0f;
-    void* jargs[] = {&p, &cols, &lift};
+    void* jargs[] = {&p, &cols};
     const uint32_t rows = p.rows < (uint32_t)cols ? p.rows : (uint32_t)cols;
-    if (cudaError_t e = launch_kernel((const void*)k_join<HD>, dim3(p.blocks, rows), dim3(HD), 0, s, true, jargs)) return e;
+    if (cudaError_t e = launch_kernel((const void*)k_join<HD>, dim3(p.blocks, rows), dim3(JOIN_THREADS / HD * HD), 0, s, true, jargs))
+      return e;
   }
   if (p.a.weights) {
-    const uint32_t units = (p.a.max_len + UNIT - 1) / UNIT, pairs = p.a.kv.n_kv_heads * p.a.kv.n_seqs;
-    uint32_t x = (16 * 148 + pairs - 1) / pairs;
-    if (x > units) x = units;
-    if (x == 0) return cudaSuccess;
-    return launch_kernel((const void*)k_weights<BF, HD, PARTS, NT>, dim3(x, p.a.kv.n_kv_heads, p.a.kv.n_seqs), dim3(THREADS), 0,
-                         s, true, args);
+    return launch_kernel((const void*)k_weights<BF, HD, PARTS, NT>, dim3(p.blocks), dim3(THREADS), 0, s, true, args);
   }
   return cudaSuccess;
 }
 template <bool BF, int HD, int PARTS>
 cudaError_t launch_nt(Plan& p, int nt, cudaStream_t s) {
-  if (nt == 1) return launch<BF, HD, PARTS, 1>(p, s);
-  if constexpr (HD <= MAX_HD_NT4)
-    if (nt == 4) return launch<BF, HD, PARTS, 4>(p, s);
-  return launch<BF, HD, PARTS, 2>(p, s);
+  return nt == 1 ? launch<BF, HD, PARTS, 1>(p, s) : nt == 2 ? launch<BF, HD, PARTS, 2>(p, s) : launch<BF, HD, PARTS, 4>(p, s);
 }
 template <bool BF, int PARTS>
 cudaError_t launch_hd(Plan& p, int nt, cudaStream_t s) {
