@@ -35,6 +35,9 @@ size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   p.step_off = pattn::UNIT % kv.page_size;
   p.min_units = 4;
   p.direct = units <= p.min_units && items <= 0x7fffffffu;
+  const uint64_t w_units = (uint64_t)kv.n_seqs * kv.n_kv_heads * (units ? units : 1);
+  const uint64_t w_resident = (uint64_t)sm_count() * pattn::WEIGHTS_RESIDENT;
+  p.weight_blocks = (uint32_t)(w_units < w_resident ? w_units : w_resident);
   if (p.direct) {
     p.blocks = (uint32_t)items;
   } else {

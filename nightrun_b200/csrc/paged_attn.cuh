@@ -41,6 +41,7 @@ constexpr int THREADS = 128, WARPS = 4;
 constexpr int TILE = 16;             // positions per warp and step
 constexpr int UNIT = TILE * WARPS;   // positions per block and step: the unit of the schedule
 // Blocks per SM, by the registers.
+constexpr int WEIGHTS_RESIDENT = 4;
 constexpr int resident(int hd, int nt) { return nt > 1 ? 2 : hd <= 32 ? 4 : 3; }
 
 // What one launch needs beside the arguments.
@@ -48,6 +49,7 @@ struct Plan {
   PagedAttnArgs a;
   uint32_t gqa, rows, row_blocks;  // query rows per KV head (gqa * n_new), blocks of 8 * NT of them
   uint32_t blocks;                 // blocks of the attention kernel
+  uint32_t weight_blocks;          // blocks of the weights' kernel
   uint32_t direct;                 // one (sequence, KV head, row block) per block: nothing is split
   uint32_t min_units;
   int4* cut;                       // [blocks]: the work that starts in this block and ends in a later one
@@ -158,30 +160,46 @@ struct VTile {
     a[2] = __byte_perm(x[2], x[3], 0x5410);
     a[3] = __byte_perm(x[2], x[3], 0x7632);
   }
+  // Whether an infinity or NaN stands among the pieces.
+  template <bool BF>
+  NRC_DEV bool odd() const {
+    constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+      for (int c = 0; c < HD / 64; c++)
+        any = any || __vcmpeq2(w[c][i].x & EXP, EXP) || __vcmpeq2(w[c][i].y & EXP, EXP) || __vcmpeq2(w[c][i].z & EXP, EXP) ||
+              __vcmpeq2(w[c][i].w & EXP, EXP);
+      if (HD % 64) any = any || __vcmpeq2(h[i].x & EXP, EXP) || __vcmpeq2(h[i].y & EXP, EXP);
+    }
+    return any;
+  }
 };
 
 // A warp's way through its tiles, every WARPS-th from `tile` on below position `end`. Where pages are whole tiles
 // (page_size % 16 == 0) one lookup, alike in all lanes, serves a tile; else each lane looks its position up.
 struct Walk {
-  const uint8_t *k, *v;    // the KV head's row 0 (in bytes), this lane's piece
+  const uint8_t *k, *v;    // the KV head's first row, this lane's pieces
   const int32_t* table;
-  int64_t row;             // byte offset of the current tile's first row (or of this lane's), -1: none
+  int64_t row;             // byte offset of the current tile's first row (or of this lane's)
   int64_t step;            // bytes between positions
   uint32_t end, pos;       // pos: of the tile looked up next (its first, or this lane's own)
   uint32_t pi, off;        // page index and offset of pos
   int32_t page;            // table[pi], read one tile ahead
-  uint32_t left;           // positions of the current tile before the end
+  uint32_t ok;             // positions of the current tile that can be read, as bits
   bool in_page;
   bool bad;                // a page outside the pool was met: tiles have to be masked by cached()
 
   NRC_DEV void fetch() { page = pos < end ? table[pi] : 0; }
   NRC_DEV void begin(const Plan& p, uint32_t b, uint32_t h, uint32_t tile, uint32_t end_, int lane) {
-    k = static_cast<const uint8_t*>(p.a.kv.k) + (int64_t)h * p.a.kv.head_stride * 2 + 16 * (lane & 3);
-    v = static_cast<const uint8_t*>(p.a.kv.v) + (int64_t)h * p.a.kv.head_stride * 2;
-    table = p.a.kv.table + (size_t)b * p.a.kv.table_stride;
+    const int g = lane >> 2, t = lane & 3;
     step = p.a.kv.pos_stride * 2;
-    end = end_;
     in_page = p.a.kv.page_size % TILE == 0;
+    k = static_cast<const uint8_t*>(p.a.kv.k) + (int64_t)h * p.a.kv.head_stride * 2 + 16 * t + (in_page ? g * step : 0);
+    v = static_cast<const uint8_t*>(p.a.kv.v) + (int64_t)h * p.a.kv.head_stride * 2 + 16 * g + (in_page ? 2 * t * step : 0);
+    table = p.a.kv.table + (size_t)b * p.a.kv.table_stride;
+    end = end_;
     bad = false;
     pos = tile * TILE + (in_page ? 0 : lane & 15);
     pi = pos / p.a.kv.page_size;
@@ -189,15 +207,17 @@ struct Walk {
     fetch();
   }
   // Makes the tile at `pos` the current one and moves on.
-  NRC_DEV void next(const Plan& p, int lane) {
-    const uint32_t tile0 = in_page ? pos : pos - (lane & 15);
-    left = tile0 < end ? min(end - tile0, (uint32_t)TILE) : 0;
+  NRC_DEV void next(const Plan& p) {
     const bool live = pos < end, found = (uint32_t)page < p.a.kv.n_pages;
-    row = live && found ? ((int64_t)page * p.a.kv.page_stride + (int64_t)off * p.a.kv.pos_stride) * 2 : -1;
-    if (__any_sync(0xffffffffu, live && !found)) {
-      if (live && !found) atomicOr(p.err, ERR_BAD_PAGE);
-      bad = true;
+    row = ((int64_t)page * p.a.kv.page_stride + (int64_t)off * p.a.kv.pos_stride) * 2;
+    if (in_page) {
+      ok = !live || !found ? 0u : end - pos < TILE ? (1u << (end - pos)) - 1u : 0xffffu;
+      if (live && !found) bad = true;
+    } else {
+      ok = __ballot_sync(0xffffffffu, live && found) & 0xffffu;
+      if (__any_sync(0xffffffffu, live && !found)) bad = true;
     }
+    if (live && !found) atomicOr(p.err, ERR_BAD_PAGE);
     pos += UNIT;
     pi += p.step_pages;
     off += p.step_off;
@@ -207,49 +227,52 @@ struct Walk {
     }
     fetch();
   }
-  // All 16 rows can be read at row + r * step.
-  NRC_DEV bool plain() const { return in_page && left == TILE && row >= 0; }
-  NRC_DEV int64_t row_of(int r) const {
-    if (in_page) return row >= 0 && (uint32_t)r < left ? row + r * step : -1;
-    return __shfl_sync(0xffffffffu, row, r);
-  }
   template <int HD>
   NRC_DEV void load_k(KTile<HD>& t, int lane) const {
     const int g = lane >> 2;
-    if (plain()) {
-      const uint8_t* p0 = k + (row + g * step);
-      const uint8_t* p1 = p0 + 8 * step;
+    const uint8_t *p0, *p1;
+    if (in_page) {
+      p0 = k + row;
+      p1 = p0 + 8 * step;
+    } else {
+      p0 = k + __shfl_sync(0xffffffffu, row, g);
+      p1 = k + __shfl_sync(0xffffffffu, row, g + 8);
+    }
+    if (ok == 0xffffu) {
 #pragma unroll
       for (int c = 0; c < HD / 32; c++) t.w[c][0] = ldg16(p0 + 64 * c), t.w[c][1] = ldg16(p1 + 64 * c);
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int64_t o = row_of(g + 8 * i);
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int c = 0; c < HD / 32; c++) t.w[c][i] = o >= 0 ? ldg16(k + o + 64 * c) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < HD / 32; c++)
+          t.w[c][i] = (ok >> (g + 8 * i)) & 1 ? ldg16((i ? p1 : p0) + 64 * c) : make_uint4(0, 0, 0, 0);
     }
   }
   template <int HD>
   NRC_DEV void load_v(VTile<HD>& t, int lane) const {
     const int g = lane >> 2, q = lane & 3;
-    if (plain()) {
-      const uint8_t* p0 = v + (row + 2 * q * step);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint8_t* pr = p0 + ((i & 1) + 8 * (i >> 1)) * step;
-#pragma unroll
-        for (int c = 0; c < HD / 64; c++) t.w[c][i] = ldg16(pr + 16 * g + 128 * c);
-        if (HD % 64) t.h[i] = ldg8(pr + 8 * g + 2 * (HD - 32));
-      }
-      return;
-    }
+    const uint8_t* pr[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int64_t o = row_of(2 * q + (i & 1) + 8 * (i >> 1));
+      const int r = (i & 1) + 8 * (i >> 1);
+      pr[i] = v + (in_page ? row + r * step : __shfl_sync(0xffffffffu, row, 2 * q + r));
+    }
+    if (ok == 0xffffu) {
 #pragma unroll
-      for (int c = 0; c < HD / 64; c++) t.w[c][i] = o >= 0 ? ldg16(v + o + 16 * g + 128 * c) : make_uint4(0, 0, 0, 0);
-      if (HD % 64) t.h[i] = o >= 0 ? ldg8(v + o + 8 * g + 2 * (HD - 32)) : make_uint2(0, 0);
+      for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int c = 0; c < HD / 64; c++) t.w[c][i] = ldg16(pr[i] + 128 * c);
+        if (HD % 64) t.h[i] = ldg8(pr[i] + 2 * (HD - 32) - 8 * g);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const bool there = (ok >> (2 * q + (i & 1) + 8 * (i >> 1))) & 1;
+#pragma unroll
+        for (int c = 0; c < HD / 64; c++) t.w[c][i] = there ? ldg16(pr[i] + 128 * c) : make_uint4(0, 0, 0, 0);
+        if (HD % 64) t.h[i] = there ? ldg8(pr[i] + 2 * (HD - 32) - 8 * g) : make_uint2(0, 0);
+      }
     }
   }
   // Which positions of a tile are cached, where a bad page was met.
@@ -389,6 +412,25 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start
 // their positions. f16 weights: up to 2^15, and with bits down to 2^-24, 2^-32 of the row's sum. UNSET: nothing seen.
 constexpr float SLACK = 7.0f, LIFT = 8.0f, UNSET = 3e38f;
 
+// Exponentials of 8 columns' scores, added to the rows' sums, as operand B of O^T.
+template <bool BF, int PARTS>
+NRC_DEV void weights_operand(uint32_t (&pb)[PARTS][2], const float (&s)[4], const float (&ref)[2], float (&l)[2]) {
+  float e[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    e[i] = exp2_fast(s[i] + ref[i & 1]);
+    l[i & 1] += e[i];
+  }
+  uint32_t lo[PARTS], hi[PARTS];
+  split2<BF, PARTS>(e[0], e[1], lo);
+  split2<BF, PARTS>(e[2], e[3], hi);
+#pragma unroll
+  for (int j = 0; j < PARTS; j++) {
+    pb[j][0] = transpose8x8(lo[j]);
+    pb[j][1] = transpose8x8(hi[j]);
+  }
+}
+
 template <bool BF, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid_constant__ Plan p) {
   constexpr int MT = HD / 16, COLS = 8 * NT;
@@ -423,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
     walk.begin(p, b, h, u0 * WARPS + warp, end, lane);
     KTile<HD> k;
     VTile<HD> v;
-    walk.next(p, lane);
+    walk.next(p);
     walk.load_k<HD>(k, lane);
     walk.load_v<HD>(v, lane);
     load_queries<BF, HD, PARTS, NT>(p, b, h, rb, qs);
@@ -451,38 +493,37 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
     };
 
     for (uint32_t p0 = (u0 * WARPS + warp) * TILE; p0 < end; p0 += UNIT) {
-      float s[NT][4], e[NT][4];
+      float s[NT][4];
       scores<BF, HD, PARTS, NT>(s, k, qs, lane);
-      walk.next(p, lane);
+      walk.next(p);
       walk.load_k<HD>(k, lane);
-      const bool whole = p0 + TILE <= all_see && !walk.bad;
-      bool grows = false;
+      const bool all = p0 + TILE <= all_see;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) e[n][i] = fmaf(s[n][i], fac[n][i & 1], ref[n][i & 1]);
-      if (!whole) {
+        for (int i = 0; i < 4; i++) s[n][i] *= fac[n][i & 1];
+      if (!all || walk.bad) {
         const uint32_t ok = walk.bad ? walk.cached(p, b, p0, lane) : 0xffffu;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const uint32_t r = g + 8 * (i >> 1);
-            if (!((ok >> r) & 1) || p0 + r >= sees(8 * n + 2 * t + (i & 1))) e[n][i] = -INFINITY;
+            if (!((ok >> r) & 1) || p0 + r >= sees(8 * n + 2 * t + (i & 1))) s[n][i] = -INFINITY;
           }
       }
+      float over = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; n++)
-        grows = grows || fmaxf(fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3])) > LIFT + SLACK;
-      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) over = fmaxf(over, fmaxf(s[n][i], s[n][i + 2]) + ref[n][i]);
+      if (__any_sync(0xffffffffu, over > LIFT + SLACK)) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float f[2];
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float x0 = e[n][i] == -INFINITY ? -INFINITY : s[n][i] * fac[n][i];
-            const float x1 = e[n][i + 2] == -INFINITY ? -INFINITY : s[n][i + 2] * fac[n][i];
-            float x = fmaxf(x0, x1);
+            float x = fmaxf(s[n][i], s[n][i + 2]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -490,8 +531,6 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
             f[i] = exp2_fast(now - ref[n][i]);
             ref[n][i] = now;
             l[n][i] *= f[i];
-            e[n][i] = x0 + now;
-            e[n][i + 2] = x1 + now;
           }
 #pragma unroll
           for (int j = 0; j < MT; j++)
@@ -499,52 +538,40 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
             for (int i = 0; i < 4; i++) acc[j][n][i] *= f[i & 1];
         }
       }
-      uint32_t pb[NT][PARTS][2];
+      // Where only some of the new tokens see a position, 0 times an infinite value must not reach the others.
+      const bool careful = !all && p.a.n_new > 1 && __any_sync(0xffffffffu, v.template odd<BF>());
+      if (!careful) {
+        uint32_t a[MT][4];
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
+        for (int j = 0; j < MT; j++) v.operand(a[j], j);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          e[n][i] = exp2_fast(e[n][i]);
-          l[n][i & 1] += e[n][i];
-        }
-        uint32_t lo[PARTS], hi[PARTS];
-        split2<BF, PARTS>(e[n][0], e[n][1], lo);
-        split2<BF, PARTS>(e[n][2], e[n][3], hi);
-#pragma unroll
-        for (int j = 0; j < PARTS; j++) {
-          pb[n][j][0] = transpose8x8(lo[j]);
-          pb[n][j][1] = transpose8x8(hi[j]);
-        }
-      }
-      if (p0 + TILE <= all_see || p.a.n_new == 1) {
-#pragma unroll
-        for (int j = 0; j < MT; j++) {
-          uint32_t a[4];
-          v.operand(a, j);
+        for (int n = 0; n < NT; n++) {
+          uint32_t pb[PARTS][2];
+          weights_operand<BF, PARTS>(pb, s[n], ref[n], l[n]);
 #pragma unroll
           for (int i = 0; i < PARTS; i++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) mma<BF>(acc[j][n], a, pb[n][i][0], pb[n][i][1]);
+            for (int j = 0; j < MT; j++) mma<BF>(acc[j][n], a[j], pb[i][0], pb[i][1]);
         }
       } else {
-        // Positions that only some of the new tokens see: 0 times an infinite value must not reach the others, so
-        // each token's rows are taken from a product with the values behind it cleared.
+        // Each token's rows are taken from a product with the values behind it cleared.
         const uint32_t tok0 = rb * COLS / p.gqa, tok1 = min(p.a.n_new, (rb * COLS + COLS - 1) / p.gqa + 1);
-        for (uint32_t tok = tok0; tok < tok1; tok++) {
-          const uint32_t behind = p.a.n_new - 1 - tok, stop = len > behind ? len - behind : 0;
-          const uint32_t at = p0 + 2 * t;
-          const uint32_t mask0 = (at < stop ? 0xffffu : 0u) | (at + 1 < stop ? 0xffff0000u : 0u);
-          const uint32_t mask1 = (at + 8 < stop ? 0xffffu : 0u) | (at + 9 < stop ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int j = 0; j < MT; j++) {
-            uint32_t a[4];
-            v.operand(a, j);
-            a[0] &= mask0, a[1] &= mask0, a[2] &= mask1, a[3] &= mask1;
+        for (int n = 0; n < NT; n++) {
+          uint32_t pb[PARTS][2];
+          weights_operand<BF, PARTS>(pb, s[n], ref[n], l[n]);
+          for (uint32_t tok = tok0; tok < tok1; tok++) {
+            const uint32_t behind = p.a.n_new - 1 - tok, stop = len > behind ? len - behind : 0, at = p0 + 2 * t;
+            const uint32_t mask0 = (at < stop ? 0xffffu : 0u) | (at + 1 < stop ? 0xffff0000u : 0u);
+            const uint32_t mask1 = (at + 8 < stop ? 0xffffu : 0u) | (at + 9 < stop ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int j = 0; j < MT; j++) {
+              uint32_t a[4];
+              v.operand(a, j);
+              a[0] &= mask0, a[1] &= mask0, a[2] &= mask1, a[3] &= mask1;
               float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int i = 0; i < PARTS; i++) mma<BF>(d, a, pb[n][i][0], pb[n][i][1]);
+              for (int i = 0; i < PARTS; i++) mma<BF>(d, a, pb[i][0], pb[i][1]);
 #pragma unroll
               for (int i = 0; i < 4; i++)
                 if ((rb * COLS + 8 * n + 2 * t + (i & 1)) / p.gqa == tok) acc[j][n][i] += d[i];
@@ -657,7 +684,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ P
 // Weights: the scores again (the same products, the same bits; they would take more memory traffic than K does), then
 // 2^(s - lse) summed over the query rows in a fixed order and added. The attention's schedule, without row blocks.
 template <bool BF, int HD, int PARTS, int NT>
-__global__ void __launch_bounds__(THREADS) k_weights(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __grid_constant__ Plan p) {
   constexpr int COLS = 8 * NT;
   __shared__ Queries<HD, PARTS, NT> qs;
   __shared__ uint64_t warp_sums[WARPS];
@@ -676,7 +703,7 @@ __global__ void __launch_bounds__(THREADS) k_weights(const __grid_constant__ Pla
       Walk walk;
       walk.begin(p, b, h, u0 * WARPS + warp, end, lane);
       KTile<HD> k;
-      walk.next(p, lane);
+      walk.next(p);
       walk.load_k<HD>(k, lane);
       load_queries<BF, HD, PARTS, NT>(p, b, h, rb, qs);
       __syncthreads();
@@ -696,7 +723,7 @@ __global__ void __launch_bounds__(THREADS) k_weights(const __grid_constant__ Pla
       for (uint32_t p0 = (u0 * WARPS + warp) * TILE; p0 < end; p0 += UNIT) {
         float s[NT][4], sum[2] = {0.0f, 0.0f};
         scores<BF, HD, PARTS, NT>(s, k, qs, lane);
-        walk.next(p, lane);
+        walk.next(p);
         walk.load_k<HD>(k, lane);
         const bool whole = p0 + TILE <= all_see && !walk.bad;
         const uint32_t ok = walk.bad ? walk.cached(p, b, p0, lane) : 0xffffu;
@@ -746,7 +773,7 @@ cudaError_t launch(Plan& p, cudaStream_t s) {
       return e;
   }
   if (p.a.weights) {
-    return launch_kernel((const void*)k_weights<BF, HD, PARTS, NT>, dim3(p.blocks), dim3(THREADS), 0, s, true, args);
+    return launch_kernel((const void*)k_weights<BF, HD, PARTS, NT>, dim3(p.weight_blocks), dim3(THREADS), 0, s, true, args);
   }
   return cudaSuccess;
 }
