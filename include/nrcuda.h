@@ -220,7 +220,7 @@ int nrc_kv_evict(const nrc_paged_kv* kv, int32_t* kept, int32_t* new_lens, float
  * (exact in 64 bits); at the first refusal a the next token is drawn from max(p_a - q_a, 0), or,
  * when every draft was taken, from p_a: the first index whose running sum, in 64 bits, exceeds
  * u[n_max] times the whole sum (p_a itself where the difference leaves nothing; token 0 where that
- * holds nothing positive either; NaN counts as nothing). tokens[s] = the a taken drafts, the drawn
+ * holds nothing positive either; NaN and infinities count as nothing). tokens[s] = the a taken drafts, the drawn
  * token, then -1; accepted[s] = a. p: [n_seqs][n_max + 1][vocab], q: [n_seqs][n_max][vocab] (NULL:
  * each draft was certain, q = 1 at it), of `dtype`, with sequence and token strides; draft: int32
  * [n_seqs][n_max] (an id outside the vocabulary is refused); u: f32 [n_seqs][n_max + 1] in [0, 1);

@@ -2,12 +2,14 @@
 //
 // Draft x_i is taken while u_i q_i(x_i) < p_i(x_i), an exact comparison in 64 bits (products of two f32 values); the
 // token behind the taken ones is the first index whose running sum of r = max(p - q, 0) (or of p) exceeds u times the
-// whole sum. The running sums are taken in 64 bits: in 32 the order of the additions would move the drawn token.
+// whole sum. The running sums are taken in 64 bits: in 32 the order of the additions would move the drawn token. (Pairs of
+// f32 with error-free sums, to save the conversions: 47 against 44 us for 160 rows of 151936. It is not the arithmetic.)
 //
 // Bound by reading one row of p (and of q): HBM for many sequences, latency for few. A cluster of blocks takes a
 // sequence, each warp a contiguous span of the row; the span sums are exchanged through distributed shared memory, and
-// only the span that holds the goal is read again, by one warp.
+// only the group of a span's tokens that holds the goal is read again, by the warp that summed it.
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include "paged.cuh"
 
@@ -16,14 +18,21 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_MAX_CLUSTER = 8;
+constexpr int VD_MAX_CLUSTER = 8;
 
-// What is left of p at one token: max(p - q, 0) after a refusal, p itself otherwise; NaN and
-// negative values count as nothing. The difference of two f32 values is formed in 64 bits.
-NRC_DEV double left_of(float p, float q) {
-  const double d = (double)p - (double)q;
-  return d > 0.0 ? d : 0.0;
-}
+// What is left of p at one token: max(p - q, 0) after a refusal, p itself otherwise; NaN, infinities and negative values
+// count as nothing. The difference of two f32 values is formed in 64 bits.
+NRC_DEV double left_of(float p, float q) { return p > q && p <= FLT_MAX ? (double)p - (double)q : 0.0; }
+
+// Two running sums of what is left.
+struct Sums {
+  double a = 0.0, b = 0.0;
+  NRC_DEV void add(float2 p, float2 q) {
+    a += left_of(p.x, q.x);
+    b += left_of(p.y, q.y);
+  }
+  NRC_DEV double value() const { return a + b; }
+};
 
 template <int DT>
 struct Row {
@@ -34,105 +43,187 @@ struct Row {
   }
 };
 
-// Sum of [t0, t1) over the warp. Rows may start anywhere: single values up to a 16-byte border of p, then 16-byte
-// pieces where q is aligned like p, single values otherwise.
-template <int DT>
-NRC_DEV double span_sum(const Row<DT>& r, uint32_t t0, uint32_t t1, int lane) {
-  constexpr uint32_t SIZE = DT == NRC_F32 ? 4 : 2, W = 16 / SIZE;
-  double s0 = 0.0, s1 = 0.0;
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(r.p), qa = reinterpret_cast<uintptr_t>(r.q);
-  if (pa % SIZE == 0 && (!r.q || (pa - qa) % 16 == 0)) {
-    const uint32_t ahead = min((uint32_t)((16 - (pa + (uint64_t)t0 * SIZE) % 16) % 16) / SIZE, t1 - t0);
-    if ((uint32_t)lane < ahead) s0 += r.at(t0 + lane);
-    t0 += ahead;
-    const uint32_t pieces = (t1 - t0) / W;
-    const uint4* pv = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.p) + (uint64_t)t0 * SIZE);
-    const uint4* qv = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.q) + (uint64_t)t0 * SIZE);
-    constexpr int U = 4;
-    for (uint32_t i0 = lane; i0 < pieces; i0 += 32 * U) {
-      uint4 x[U], y[U];
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const uint32_t i = i0 + 32 * k;
-        x[k] = y[k] = make_uint4(0, 0, 0, 0);
-        if (i < pieces) {
-          x[k] = __ldg(pv + i);
-          if (r.q) y[k] = __ldg(qv + i);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const uint32_t first = t0 + (i0 + 32 * k) * W;
-#pragma unroll
-        for (uint32_t e = 0; e < W; e++) {
-          const float q = r.q ? load_as_f32(&y[k], e, DT) : (int32_t)(first + e) == r.certain ? 1.0f : 0.0f;
-          const double d = left_of(load_as_f32(&x[k], e, DT), q);
-          if (e & 1)
-            s1 += d;
-          else
-            s0 += d;
-        }
-      }
-    }
-    t0 += pieces * W;
-    if (t0 + lane < t1) s0 += r.at(t0 + lane);
-  } else {
-    constexpr int U = 8;
-    for (uint32_t i0 = t0 + lane; i0 < t1; i0 += 32 * U)
-#pragma unroll
-      for (int k = 0; k < U; k++)
-        if (i0 + 32 * k < t1) s0 += r.at(i0 + 32 * k);
-  }
-  double s = s0 + s1;
+NRC_DEV double warp_sum(double s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
+// How a warp walks a span of tokens: single values up to the first 16-byte border of p (`ahead` of them), then batches of
+// 32 * U pieces of 16 bytes where q is aligned like p, of 64 * U single values otherwise, then what is left over.
+// FINE groups of `group` batches keep sums of their own, the first with what is ahead, the last with the rest.
+constexpr int FINE = 8;
+template <int DT, int U>
+struct Span {
+  static constexpr uint32_t SIZE = DT == NRC_F32 ? 4 : 2, W = 16 / SIZE;
+  uint32_t t0, t1, ahead, batch, batches, group;
+  bool wide;
+  NRC_DEV Span(const Row<DT>& r, uint32_t a, uint32_t b) : t0(a), t1(b) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(r.p) + (uint64_t)t0 * SIZE, qa = reinterpret_cast<uintptr_t>(r.q);
+    wide = !r.q || (reinterpret_cast<uintptr_t>(r.p) - qa) % 16 == 0;
+    ahead = wide ? min((uint32_t)((16 - pa % 16) % 16) / SIZE, t1 - t0) : 0;
+    batch = wide ? 32 * U * W : 64 * U;
+    batches = (t1 - t0 - ahead + batch - 1) / batch;
+    group = (batches + FINE - 1) / FINE;
+  }
+  // The tokens of group f.
+  NRC_DEV uint32_t begin(uint32_t f) const {
+    return f == 0 ? t0 : (uint32_t)min((uint64_t)t0 + ahead + (uint64_t)f * group * batch, (uint64_t)t1);
+  }
+};
+
+// Sums of a span's groups into fine[], and of the whole.
+template <int DT, int U>
+NRC_DEV double span_sum(const Row<DT>& r, const Span<DT, U>& sp, double* fine, int lane) {
+  constexpr uint32_t W = Span<DT, U>::W;
+  double all = 0.0, edge = (uint32_t)lane < sp.ahead ? r.at(sp.t0 + lane) : 0.0;
+  const uint32_t a0 = sp.t0 + sp.ahead;
+  const uint4* pv = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.p) + (uint64_t)a0 * Span<DT, U>::SIZE);
+  const uint4* qv = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.q) + (uint64_t)a0 * Span<DT, U>::SIZE);
+  Sums s;
+  uint32_t f = 0, in_group = 0;
+  for (uint32_t i = 0; i < sp.batches; i++) {
+    const uint32_t a = a0 + i * sp.batch;
+    if (sp.wide) {
+      uint4 x[U], y[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const uint32_t piece = (i * U + k) * 32 + lane;
+        x[k] = y[k] = make_uint4(0, 0, 0, 0);
+        if (a0 + (piece + 1) * W <= sp.t1) {
+          x[k] = __ldg(pv + piece);
+          if (r.q) y[k] = __ldg(qv + piece);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const uint32_t t = a + (lane + 32 * k) * W;
+#pragma unroll
+        for (uint32_t e = 0; e < W; e += 2) {
+          float2 q = make_float2(load_as_f32(&y[k], e, DT), load_as_f32(&y[k], e + 1, DT));
+          if (!r.q) q = make_float2((int32_t)(t + e) == r.certain ? 1.0f : 0.0f, (int32_t)(t + e + 1) == r.certain ? 1.0f : 0.0f);
+          s.add(make_float2(load_as_f32(&x[k], e, DT), load_as_f32(&x[k], e + 1, DT)), q);
+        }
+        if (t < sp.t1 && t + W > sp.t1)  // the piece that the span cuts
+          for (uint32_t u = t; u < sp.t1; u++) edge += r.at(u);
+      }
+    } else {
+      float p[2 * U], q[2 * U];
+#pragma unroll
+      for (int k = 0; k < 2 * U; k++) {
+        const uint32_t t = a + lane + 32 * k;
+        p[k] = t < sp.t1 ? load_as_f32(r.p, t, DT) : 0.0f;
+        q[k] = t < sp.t1 ? load_as_f32(r.q, t, DT) : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 2 * U; k += 2) s.add(make_float2(p[k], p[k + 1]), make_float2(q[k], q[k + 1]));
+    }
+    if (++in_group == sp.group || i + 1 == sp.batches) {
+      const double g = warp_sum(s.value() + edge);
+      if (lane == 0) fine[f] = g;
+      all += g;
+      s = Sums();
+      edge = 0.0;
+      in_group = 0;
+      f++;
+    }
+  }
+  if (sp.batches == 0) {
+    all = warp_sum(edge);
+    if (lane == 0) fine[0] = all;
+    f = 1;
+  }
+  if ((uint32_t)lane >= f && lane < FINE) fine[lane] = 0.0;
+  __syncwarp();
+  return all;
+}
+
 // First index of [t0, t1) whose running sum, begun at `before`, exceeds goal; where rounding leaves none, the last one
-// that holds anything.
+// that holds anything. A lane takes 4 neighbours at a time, the next ones on their way.
 template <int DT>
 NRC_DEV uint32_t span_find(const Row<DT>& r, uint32_t t0, uint32_t t1, double before, double goal, int lane) {
-  const uint32_t per = (t1 - t0 + 31) / 32, a = min(t0 + lane * per, t1), b = min(a + per, t1);
-  double s = 0.0;
-  int last = -1;
-#pragma unroll 8
-  for (uint32_t t = a; t < b; t++) {
-    const double d = r.at(t);
-    s += d;
-    if (d > 0.0) last = (int)t;
+  float p[4], q[4];
+  auto fetch = [&](uint32_t t) {
+#pragma unroll
+    for (int e = 0; e < 4; e++, t++) {
+      p[e] = t < t1 ? load_as_f32(r.p, t, DT) : 0.0f;
+      q[e] = t < t1 && r.q ? load_as_f32(r.q, t, DT) : (int32_t)t == r.certain ? 1.0f : 0.0f;
+    }
+  };
+  int last = 0;
+  fetch(t0 + 4 * lane);
+  for (; t0 < t1; t0 += 128) {
+    const int t = (int)(t0 + 4 * lane);
+    double v[4], own = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      v[e] = left_of(p[e], q[e]);
+      own += v[e];
+    }
+    fetch(t0 + 128 + 4 * lane);
+    double run = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += y;
+    }
+    double prev = __shfl_up_sync(0xffffffffu, run, 1);
+    prev = before + (lane ? prev : 0.0);
+    int found = -1, mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      prev += v[e];
+      if (v[e] > 0.0) mine = t + e;
+      if (found < 0 && v[e] > 0.0 && prev > goal) found = t + e;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, found >= 0), some = __ballot_sync(0xffffffffu, own > 0.0);
+    if (over) return (uint32_t)__shfl_sync(0xffffffffu, found, __ffs(over) - 1);
+    if (some) last = __shfl_sync(0xffffffffu, mine, 31 - __clz(some));
+    before += __shfl_sync(0xffffffffu, run, 31);
   }
-  double run = s;
+  return (uint32_t)last;
+}
+
+// The span whose running sum first exceeds goal, and the running sum before it; where rounding leaves none, the last that
+// holds anything (before: -inf); -1 if none does. One warp; sums in index order, each lane `n / 32` of them.
+NRC_DEV int pick_span(const double* sums, uint32_t n, double goal_of_total, double* total, double* before, int lane) {
+  const uint32_t each = (n + 31) / 32, i0 = min(lane * each, n), i1 = min(i0 + each, n);
+  double t = 0.0;
+  for (uint32_t i = i0; i < i1; i++) t += sums[i];
+  double run = t;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double y = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += y;
   }
-  run += before;
-  const unsigned over = __ballot_sync(0xffffffffu, run > goal), some = __ballot_sync(0xffffffffu, last >= 0);
-  if (over) {
-    const int who = __ffs(over) - 1;
-    double prev = __shfl_up_sync(0xffffffffu, run, 1);
-    if (lane == 0) prev = before;
-    int found = last;
-    if (lane == who)
-      for (uint32_t t = a; t < b; t++) {
-        prev += r.at(t);
-        if (prev > goal) {
-          found = (int)t;
-          break;
-        }
-      }
-    found = __shfl_sync(0xffffffffu, found, who);
-    if (found >= 0) return (uint32_t)found;
+  *total = __shfl_sync(0xffffffffu, run, 31);
+  const double goal = goal_of_total * *total;
+  double at = __shfl_up_sync(0xffffffffu, run, 1);
+  if (lane == 0) at = 0.0;
+  int over = -1, last = -1;
+  double at_over = 0.0;
+  for (uint32_t i = i0; i < i1; i++) {
+    const double v = sums[i];
+    if (over < 0 && at + v > goal) over = (int)i, at_over = at;
+    if (v > 0.0) last = (int)i;
+    at += v;
   }
-  return some ? (uint32_t)__shfl_sync(0xffffffffu, last, 31 - __clz(some)) : 0u;
+  const unsigned any_over = __ballot_sync(0xffffffffu, over >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
+  if (any_over) {
+    const int who = __ffs(any_over) - 1;
+    *before = __shfl_sync(0xffffffffu, at_over, who);
+    return __shfl_sync(0xffffffffu, over, who);
+  }
+  *before = -INFINITY;
+  return any ? __shfl_sync(0xffffffffu, last, 31 - __clz(any)) : -1;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(VD_THREADS) k_verify_draft(const VerifyArgs a) {
+// U: 16-byte pieces of each row that a lane keeps in flight.
+template <int DT, int WARPS, int U>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 5 : 2) k_verify_draft(const VerifyArgs a) {
   constexpr uint32_t SIZE = DT == NRC_F32 ? 4 : 2;
-  __shared__ double sums[2][VD_MAX_CLUSTER * VD_WARPS];  // every span's, in each block of the cluster
+  __shared__ double sums[2][VD_MAX_CLUSTER * WARPS];  // every span's, in each block of the cluster
+  __shared__ double fine[WARPS][FINE];                // the groups of this block's spans
   __shared__ uint32_t taken_s;
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -140,19 +231,19 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify_draft(const VerifyArgs a)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {
     // All drafts at once; the first that is refused counts.
-    int nd = a.n_draft ? a.n_draft[b] : (int)m;
-    nd = nd < 0 ? 0 : nd > (int)m ? (int)m : nd;
+    const int asked = a.n_draft ? a.n_draft[b] : (int)m, nd = asked < 0 ? 0 : asked > (int)m ? (int)m : asked;
     int taken = nd;
-    for (int i0 = 0; i0 < nd; i0 += 32) {
+    for (int i0 = 0; i0 < (int)m; i0 += 32) {
       const int i = i0 + lane;
       bool refuse = false;
-      if (i < nd) {
+      if (i < (int)m) {
         const int32_t x = a.draft[(size_t)b * m + i];
-        refuse = true;
-        if (x >= 0 && (uint32_t)x < a.vocab) {
+        const float u = a.u[(size_t)b * (m + 1) + i];
+        refuse = i < nd;
+        if (refuse && x >= 0 && (uint32_t)x < a.vocab) {
           const float px = load_as_f32(a.p, (int64_t)b * a.p_seq + (int64_t)i * a.p_token + x, DT);
           const float qx = a.q ? load_as_f32(a.q, (int64_t)b * a.q_seq + (int64_t)i * a.q_token + x, DT) : 1.0f;
-          refuse = !((double)a.u[(size_t)b * (m + 1) + i] * (double)qx < (double)px);
+          refuse = !((double)u * (double)qx < (double)px);
         }
       }
       const unsigned no = __ballot_sync(0xffffffffu, refuse);
@@ -171,75 +262,73 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify_draft(const VerifyArgs a)
   row.q = refused && a.q ? static_cast<const uint8_t*>(a.q) + ((int64_t)b * a.q_seq + (int64_t)taken * a.q_token) * SIZE
                          : nullptr;
   row.certain = refused && !a.q ? a.draft[(size_t)b * m + taken] : -1;
+  const float u = a.u[(size_t)b * (m + 1) + m];
 
   // Spans of whole 16-byte pieces (counted from the row's start), in index order over blocks and warps.
-  const uint32_t spans = blocks * VD_WARPS;
-  uint32_t per = (a.vocab + spans - 1) / spans;
-  per = (per + 7) & ~7u;
+  const uint32_t spans = blocks * WARPS, per = ((a.vocab + spans - 1) / spans + 7) & ~7u;
   auto begin = [&](uint32_t i) { return (uint32_t)min((uint64_t)i * per, (uint64_t)a.vocab); };
-  const uint32_t mine = rank * VD_WARPS + warp;
+  const uint32_t mine = rank * WARPS + warp;
+  double total, before;
+  int owner;
   for (int round = 0;; round++) {
-    const double s = span_sum<DT>(row, begin(mine), begin(mine + 1), lane);
+    const double s = span_sum<DT, U>(row, Span<DT, U>(row, begin(mine), begin(mine + 1)), fine[warp], lane);
     if ((uint32_t)lane < blocks) *cluster.map_shared_rank(&sums[round][mine], lane) = s;
     cluster.sync();
-    if (warp != 0 && round == 1) return;
-    // Each block's warps look for the goal alike: the running sums of the spans, `each` of them per lane.
-    const uint32_t each = (spans + 31) / 32;
-    double t = 0.0;
-    for (uint32_t i = lane * each; i < min((lane + 1) * each, spans); i++) t += sums[round][i];
-    double run = t;
+    // Every warp of the cluster reads the same sums and decides alike.
+    owner = pick_span(sums[round], spans, (double)u, &total, &before, lane);
+    if (owner >= 0 || !refused || round) break;
+    row.q = nullptr;  // the difference leaves nothing: p itself
+    row.certain = -1;
+  }
+  uint32_t token = 0;
+  if (owner < 0) {
+    if (rank || warp) return;  // p holds nothing either
+  } else {
+    if ((uint32_t)owner != mine) return;
+    // The owner's groups, then the tokens of the one that holds the goal.
+    const Span<DT, U> sp(row, begin(mine), begin(mine + 1));
+    const double goal = (double)u * total;
+    const double f = lane < FINE ? fine[warp][lane] : 0.0;
+    double run = f;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += y;
     }
-    const double total = __shfl_sync(0xffffffffu, run, 31);
-    if (!(total > 0.0) && refused && round == 0) {  // the difference leaves nothing: p itself (every block agrees)
-      row.q = nullptr;
-      row.certain = -1;
-      continue;
-    }
-    if (warp != 0) return;
-    const double goal = (double)a.u[(size_t)b * (m + 1) + m] * total;
-    double before = run - t;
-    // The lane's spans one by one: the first whose running sum exceeds the goal, and the last that holds anything.
-    int over = -1, last = -1;
-    double at_over = 0.0, x = __shfl_up_sync(0xffffffffu, run, 1);
-    before = lane ? x : 0.0;
-    for (uint32_t i = lane * each; i < min((lane + 1) * each, spans); i++) {
-      const double v = sums[round][i];
-      if (over < 0 && before + v > goal) over = (int)i, at_over = before;
-      if (v > 0.0) last = (int)i;
-      before += v;
-    }
-    const unsigned any_over = __ballot_sync(0xffffffffu, over >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
-    uint32_t token = 0, owner = 0;
-    if (any_over) {
-      const int who = __ffs(any_over) - 1;
-      owner = (uint32_t)__shfl_sync(0xffffffffu, over, who);
-      at_over = __shfl_sync(0xffffffffu, at_over, who);
-    } else if (any) {  // rounding, or u not below 1: the last token that holds anything
-      owner = (uint32_t)__shfl_sync(0xffffffffu, last, 31 - __clz(any));
-      at_over = -INFINITY;
-    }
-    if (owner / VD_WARPS != rank) return;
-    if (any_over || any) token = span_find<DT>(row, begin(owner), begin(owner + 1), at_over, goal, lane);
-    for (uint32_t i = lane; i <= m; i += 32)
-      a.tokens[(size_t)b * (m + 1) + i] = i < taken ? a.draft[(size_t)b * m + i] : i == taken ? (int32_t)token : -1;
-    if (lane == 0) a.accepted[b] = (int32_t)taken;
-    return;
+    run += before;
+    const unsigned over = __ballot_sync(0xffffffffu, run > goal), some = __ballot_sync(0xffffffffu, f > 0.0);
+    const int pick = over ? __ffs(over) - 1 : 31 - __clz(some);
+    double at = __shfl_up_sync(0xffffffffu, run, 1);
+    if (lane == 0) at = before;
+    at = over ? __shfl_sync(0xffffffffu, at, pick) : -INFINITY;
+    token = span_find<DT>(row, sp.begin(pick), sp.begin(pick + 1), at, goal, lane);
   }
+  for (uint32_t i = lane; i <= m; i += 32)
+    a.tokens[(size_t)b * (m + 1) + i] = i < taken ? a.draft[(size_t)b * m + i] : i == taken ? (int32_t)token : -1;
+  if (lane == 0) a.accepted[b] = (int32_t)taken;
+}
+
+template <int DT>
+const void* variant(bool many) {
+  return many ? (const void*)k_verify_draft<DT, 8, 2> : (const void*)k_verify_draft<DT, 16, 4>;
 }
 
 }  // namespace
 
 cudaError_t verify_draft_run(const VerifyArgs& a, cudaStream_t s) {
-  // Blocks per sequence: as many as give each warp some 512 tokens.
+  // All blocks should be resident at once, or the fixed latency of a block (four dependent reads and the cluster's
+  // barrier, some 5 us) is paid again: up to 18 sequences in clusters of 8 wide blocks, at most one per SM; more in
+  // narrower blocks, five per SM, in clusters that shrink as the sequences grow in number (640 of the 740 places: clusters
+  // do not straddle the SM groups). 37 sequences of 100352, f16: 17.5 us in wide blocks, 13.7 us in narrow ones; 160
+  // of 151936, f32: 56 us in clusters of 8, 44 us of 4.
+  const bool many = (uint64_t)a.n_seqs * VD_MAX_CLUSTER > 148;
+  const uint32_t warps = many ? 8 : 16;
   uint32_t blocks = 1;
-  while (blocks < VD_MAX_CLUSTER && (uint64_t)blocks * VD_WARPS * 512 < a.vocab) blocks *= 2;
+  while (blocks < VD_MAX_CLUSTER && (uint64_t)blocks * warps * 512 < a.vocab && (uint64_t)a.n_seqs * blocks * 2 <= 640)
+    blocks *= 2;  // and a warp has some 512 tokens
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.n_seqs * blocks);
-  cfg.blockDim = dim3(VD_THREADS);
+  cfg.blockDim = dim3(32 * warps);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -250,9 +339,7 @@ cudaError_t verify_draft_run(const VerifyArgs& a, cudaStream_t s) {
   cfg.numAttrs = 1;
   VerifyArgs aa = a;
   void* args[] = {&aa};
-  const void* fn = a.dtype == NRC_F32   ? (const void*)k_verify_draft<NRC_F32>
-                   : a.dtype == NRC_F16 ? (const void*)k_verify_draft<NRC_F16>
-                                        : (const void*)k_verify_draft<NRC_BF16>;
+  const void* fn = a.dtype == NRC_F32 ? variant<NRC_F32>(many) : a.dtype == NRC_F16 ? variant<NRC_F16>(many) : variant<NRC_BF16>(many);
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 

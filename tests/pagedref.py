@@ -140,11 +140,12 @@ def verify(p, q, draft, u, n_draft):
                 break
             tokens[s, a] = x
             a += 1
-        row = np.where(p[s, a] > 0, p[s, a], 0.0)
+        row = np.where((p[s, a] > 0) & np.isfinite(p[s, a]), p[s, a], 0.0)
         left = row
         if a < most:
             sub = q[s, a] if q is not None else (np.arange(vocab) == int(draft[s, a])).astype(np.float64)
-            d = p[s, a] - sub
+            with np.errstate(invalid="ignore"):
+                d = np.where(np.isfinite(p[s, a]), p[s, a], 0.0) - sub
             left = np.where(d > 0, d, 0.0)
             if not (left > 0).any():
                 left = row

@@ -416,6 +416,7 @@ def test_verify_draft_edges(K):
     p[5, 0, ::3], q[5, 0, 1::3] = NAN, NAN
     draft[5, 0] = 3
     p[6, 0] = -p[6, 0]
+    p[6, 1:, 5], q[6, 1:, 9], p[8, 0, 40] = float("inf"), float("inf"), float("inf")
     u[7], u[8] = 0.0, 1.0 - 2.0 ** -24
     check_verify(K, p, q, draft, u, None)
     check_verify(K, p, None, draft, u, None)
