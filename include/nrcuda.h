@@ -179,32 +179,55 @@ int nrc_rope_freqs_yarn(float* out_host, float* mscale, size_t rot_dim, float th
 /* rope::apply (crates/nr-tensor/src/rope.rs:49-65) of new tokens at their own positions, and the
  * append of infer.rs:536-551, over pages. For token t and pair i < rot_dim/2 of every head of q and k
  * (style 0: values 2i, 2i+1; style 1: i, i + rot_dim/2; values from rot_dim on pass unchanged)
- *   (a, b) -> mscale * (a cos - b sin, a sin + b cos),  angle = pos[t] * freqs_dev[i],
+ *   (a, b) -> mscale * (a cos - b sin, a sin + b cos),  angle = pos[t] * freqs[i],
  * the angle in 64 bits and the rest in f32, rounded once to the output's type (nearest even). q goes
  * to q_out (q itself is allowed), k and v to slot[t] of sequence seq[t] (slot < 0: not cached).
- * q: [tokens][n_heads][head_dim], k and v: [tokens][kv heads][head_dim], of `dtype`, with token and
- * head strides; pos, seq, slot: int32 [tokens]. No two tokens of a call share (seq, slot). */
-int nrc_rope_append(const nrc_paged_kv* kv, void* q_out, int64_t qo_token, int64_t qo_head, const void* q,
-                    int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
-                    int64_t v_token, int64_t v_head, int dtype, size_t tokens, size_t n_heads, const float* freqs_dev,
-                    size_t rot_dim, float mscale, int style, const int32_t* pos, const int32_t* seq,
-                    const int32_t* slot, void* stream);
+ * q, q_out: [tokens][n_heads][head_dim], k and v: [tokens][kv heads][head_dim], of `dtype`; pos, seq,
+ * slot: int32 [tokens]. No two tokens of a call share (seq, slot). */
+typedef struct nrc_rope_args {
+  void* q_out;
+  int64_t qo_token, qo_head; /* strides */
+  const void* q;
+  int64_t q_token, q_head;
+  const void* k;
+  int64_t k_token, k_head;
+  const void* v;
+  int64_t v_token, v_head;
+  const float* freqs; /* device, rot_dim/2 values */
+  const int32_t* pos;
+  const int32_t* seq;
+  const int32_t* slot;
+  uint64_t tokens, n_heads, rot_dim;
+  int32_t dtype, style;
+  float mscale;
+  uint32_t reserved;
+} nrc_rope_args;
+int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* args, void* stream);
 /* Attention (infer.rs:553-572) of the newest n_new tokens of every sequence over its pages. lens[s]
  * counts the cached positions, the new tokens' own among them; token i of n_new sees the positions
  * before lens[s] - (n_new - 1 - i); one that sees nothing gets zeros. Per query head
  *   out = sum_t p_t V_t,  p = softmax(scale * q . K_t),
  * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into as
  * many cache-typed parts as hold all the bits of `dtype`. q and out: [n_seqs][n_new][n_heads]
- * [head_dim] of `dtype`, each with sequence, token and head strides. weights (or NULL): f32
- * [n_seqs][kv heads][weights_len]; the weight that a position received from all the query heads of
- * the KV head and all new tokens is added to it. max_len: no sequence is longer (0: the table's
- * width). workspace: nrc_attn_paged_workspace bytes, 16-byte aligned, used by one call at a time. */
+ * [head_dim] of `dtype`; lens: int32 [n_seqs]. weights (or NULL): f32 [n_seqs][kv heads][weights_len];
+ * the weight that a position received from all the query heads of the KV head and all new tokens is
+ * added to it. max_len: no sequence is longer (0: the table's width). workspace:
+ * nrc_attn_paged_workspace bytes, 16-byte aligned, used by one call at a time. */
+typedef struct nrc_attn_args {
+  void* out;
+  int64_t o_seq, o_token, o_head; /* strides */
+  const void* q;
+  int64_t q_seq, q_token, q_head;
+  const int32_t* lens;
+  float* weights;
+  void* workspace;
+  uint64_t workspace_bytes, weights_len, max_len, n_new, n_heads;
+  int32_t dtype;
+  float scale;
+} nrc_attn_args;
 int nrc_attn_paged_workspace(const nrc_paged_kv* kv, size_t n_new, size_t n_heads, int with_weights, size_t max_len,
                              size_t* out_bytes);
-int nrc_attn_paged(const nrc_paged_kv* kv, void* out, int64_t o_seq, int64_t o_token, int64_t o_head, const void* q,
-                   int64_t q_seq, int64_t q_token, int64_t q_head, int dtype, size_t n_new, size_t n_heads,
-                   const int32_t* lens, float scale, float* weights, size_t weights_len, size_t max_len,
-                   void* workspace, size_t workspace_bytes, void* stream);
+int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* args, void* stream);
 /* Eviction: every sequence longer than `budget` keeps, for each KV head, its first `sinks` and latest
  * `recent` positions and the others of largest weight (ties: the earlier one; NaN counts as the
  * smallest), budget in all. The kept rows of K and V move to the slots 0..budget-1 in their order, in

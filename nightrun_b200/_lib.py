@@ -100,9 +100,9 @@ SIGNATURES = [
     ("nrc_rope_freqs", I, [P, S, F, F, F, F, F]),
     ("nrc_rope_apply", I, [P, S, S, P, S, I, P]),
     ("nrc_rope_freqs_yarn", I, [P, P, S, F, F, F, F, F]),
-    ("nrc_rope_append", I, [P] + [P, L, L] * 4 + [I, S, S, P, S, F, I, P, P, P, P]),
+    ("nrc_rope_append", I, [P, P, P]),
     ("nrc_attn_paged_workspace", I, [P, S, S, I, S, C.POINTER(S)]),
-    ("nrc_attn_paged", I, [P, P, L, L, L, P, L, L, L, I, S, S, P, F, P, S, S, P, S, P]),
+    ("nrc_attn_paged", I, [P, P, P]),
     ("nrc_kv_evict", I, [P, P, P, P, P, P, S, S, S, S, P]),
     ("nrc_verify_draft", I, [P, P, P, L, L, P, L, L, I, S, S, S, P, P, P, P]),
     ("nrc_model_load", I, [P, S, I, I, C.POINTER(P)]),

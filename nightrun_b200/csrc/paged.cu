@@ -19,6 +19,10 @@ __device__ unsigned g_paged_err;
 // three: 59 against 47 us for 8192 tokens of 48 heads of 128, f16.)
 constexpr int ROPE_THREADS = 128, ROPE_BLOCKS = 12;
 
+struct RopeAppendArgs : nrc_rope_args {
+  nrc_paged_kv kv;
+};
+
 template <int BYTES>
 struct Bits;
 template <>
@@ -59,7 +63,7 @@ NRC_DEV void turn(float& x, float& y, float2 r) {
 template <int DT, int W>
 __global__ void __launch_bounds__(ROPE_THREADS, ROPE_BLOCKS) k_rope_append_paged(const RopeAppendArgs a) {
   __shared__ float2 cs[64];  // cosine and sine of each pair (head_dim <= 128)
-  const uint32_t t = blockIdx.x, hd = a.kv.head_dim, half = a.rot_dim / 2, hq = a.n_heads, hk = a.kv.n_kv_heads;
+  const uint32_t t = blockIdx.x, hd = a.kv.head_dim, half = (uint32_t)a.rot_dim / 2, hq = (uint32_t)a.n_heads, hk = a.kv.n_kv_heads;
   // The item's head (query heads, then K's, then V's), its place in it, and its two groups of W values: halves pair their
   // first half / W items, the others hold what is not rotated.
   const uint32_t per_head = hd / (2 * W), item = blockIdx.y * ROPE_THREADS + threadIdx.x;
@@ -131,8 +135,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, ROPE_BLOCKS) k_rope_append_paged
 
 template <int DT, int W>
 cudaError_t launch_rope(const RopeAppendArgs& a, cudaStream_t s) {
-  const uint32_t items = (a.n_heads + 2 * a.kv.n_kv_heads) * (a.kv.head_dim / (2 * W));
-  k_rope_append_paged<DT, W><<<dim3(a.tokens, (items + ROPE_THREADS - 1) / ROPE_THREADS), ROPE_THREADS, 0, s>>>(a);
+  const uint32_t items = ((uint32_t)a.n_heads + 2 * a.kv.n_kv_heads) * (a.kv.head_dim / (2 * W));
+  k_rope_append_paged<DT, W><<<dim3((uint32_t)a.tokens, (items + ROPE_THREADS - 1) / ROPE_THREADS), ROPE_THREADS, 0, s>>>(a);
   return cudaGetLastError();
 }
 template <int DT>
@@ -331,7 +335,10 @@ __global__ void __launch_bounds__(1024) k_evict_move(const EvictArgs a) {
 
 }  // namespace
 
-cudaError_t rope_append_paged_run(const RopeAppendArgs& a, cudaStream_t s) {
+cudaError_t rope_append_paged_run(const nrc_paged_kv& kv, const nrc_rope_args& r, cudaStream_t s) {
+  RopeAppendArgs a;
+  static_cast<nrc_rope_args&>(a) = r;
+  a.kv = kv;
   const uint32_t size = a.dtype == NRC_F32 ? 4 : 2;
   // Every bit below the access width is 0 in what all accesses start from (the pages' strides are checked already).
   uint64_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |

@@ -53,18 +53,7 @@ NRC_DEV int64_t paged_row(const nrc_paged_kv& kv, uint32_t seq, uint32_t slot) {
   return (int64_t)page * kv.page_stride + (int64_t)off * kv.pos_stride;
 }
 
-struct RopeAppendArgs {
-  nrc_paged_kv kv;
-  void* q_out;
-  const void *q, *k, *v;
-  int64_t qo_token, qo_head, q_token, q_head, k_token, k_head, v_token, v_head;
-  const float* freqs;
-  const int32_t *pos, *seq, *slot;
-  uint32_t tokens, n_heads, rot_dim;
-  int dtype, style;
-  float mscale;
-};
-cudaError_t rope_append_paged_run(const RopeAppendArgs& a, cudaStream_t s);
+cudaError_t rope_append_paged_run(const nrc_paged_kv& kv, const nrc_rope_args& r, cudaStream_t s);
 
 struct EvictArgs {
   nrc_paged_kv kv;

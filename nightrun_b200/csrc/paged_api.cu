@@ -67,33 +67,21 @@ int nrc_rope_freqs_yarn(float* out, float* mscale, size_t rot_dim, float theta, 
   return NRC_OK;
 }
 
-int nrc_rope_append(const nrc_paged_kv* kv, void* q_out, int64_t qo_token, int64_t qo_head, const void* q,
-                    int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
-                    int64_t v_token, int64_t v_head, int dtype, size_t tokens, size_t n_heads, const float* freqs,
-                    size_t rot_dim, float mscale, int style, const int32_t* pos, const int32_t* seq,
-                    const int32_t* slot, void* stream) {
+int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* r, void* stream) {
   if (int rc = check_kv(kv)) return rc;
-  if (!float_type(dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", dtype);
-  if (style != 0 && style != 1) return nrc_fail_api(NRC_ERR_INVALID, "style %d", style);
-  if (rot_dim % 2 || rot_dim > kv->head_dim) return nrc_fail_api(NRC_ERR_INVALID, "rot_dim %zu", rot_dim);
-  if (tokens > 0x7fffffff || n_heads > 16384) return nrc_fail_api(NRC_ERR_INVALID, "shape too large");
-  if (tokens == 0) return NRC_OK;
-  if ((n_heads && (!q_out || !q)) || !k || !v || !pos || !seq || !slot || (rot_dim && !freqs))
+  if (!r) return nrc_fail_api(NRC_ERR_INVALID, "null arguments");
+  if (!float_type(r->dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", r->dtype);
+  if (r->style != 0 && r->style != 1) return nrc_fail_api(NRC_ERR_INVALID, "style %d", r->style);
+  if (r->rot_dim % 2 || r->rot_dim > kv->head_dim)
+    return nrc_fail_api(NRC_ERR_INVALID, "rot_dim %llu", (unsigned long long)r->rot_dim);
+  if (r->tokens > 0x7fffffff || r->n_heads > 16384) return nrc_fail_api(NRC_ERR_INVALID, "shape too large");
+  if (r->tokens == 0) return NRC_OK;
+  if ((r->n_heads && (!r->q_out || !r->q)) || !r->k || !r->v || !r->pos || !r->seq || !r->slot || (r->rot_dim && !r->freqs))
     return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
-  if (!aligned(q, dtype) || !aligned(k, dtype) || !aligned(v, dtype) || !aligned(q_out, dtype) ||
-      !aligned4(freqs, pos, seq, slot))
+  if (!aligned(r->q, r->dtype) || !aligned(r->k, r->dtype) || !aligned(r->v, r->dtype) || !aligned(r->q_out, r->dtype) ||
+      !aligned4(r->freqs, r->pos, r->seq, r->slot))
     return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
-  RopeAppendArgs a{};
-  a.kv = *kv;
-  a.q_out = q_out;
-  a.q = q, a.k = k, a.v = v;
-  a.qo_token = qo_token, a.qo_head = qo_head, a.q_token = q_token, a.q_head = q_head;
-  a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
-  a.freqs = freqs;
-  a.pos = pos, a.seq = seq, a.slot = slot;
-  a.tokens = (uint32_t)tokens, a.n_heads = (uint32_t)n_heads, a.rot_dim = (uint32_t)rot_dim;
-  a.dtype = dtype, a.style = style, a.mscale = mscale;
-  return cuda_rc(rope_append_paged_run(a, static_cast<cudaStream_t>(stream)), "rope_append");
+  return cuda_rc(rope_append_paged_run(*kv, *r, static_cast<cudaStream_t>(stream)), "rope_append");
 }
 
 static int check_attn(const nrc_paged_kv* kv, size_t n_new, size_t n_heads, size_t* max_len) {
@@ -114,36 +102,35 @@ int nrc_attn_paged_workspace(const nrc_paged_kv* kv, size_t n_new, size_t n_head
   return NRC_OK;
 }
 
-int nrc_attn_paged(const nrc_paged_kv* kv, void* out, int64_t o_seq, int64_t o_token, int64_t o_head, const void* q,
-                   int64_t q_seq, int64_t q_token, int64_t q_head, int dtype, size_t n_new, size_t n_heads,
-                   const int32_t* lens, float scale, float* weights, size_t weights_len, size_t max_len,
-                   void* workspace, size_t workspace_bytes, void* stream) {
-  if (int rc = check_attn(kv, n_new, n_heads, &max_len)) return rc;
-  if (!float_type(dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", dtype);
-  if (!isfinite(scale)) return nrc_fail_api(NRC_ERR_INVALID, "scale is not finite");
-  if (weights && (weights_len == 0 || weights_len > 0x7fffffff))
-    return nrc_fail_api(NRC_ERR_INVALID, "weights of length %zu", weights_len);
+int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* r, void* stream) {
+  if (!r) return nrc_fail_api(NRC_ERR_INVALID, "null arguments");
+  size_t max_len = r->max_len;
+  if (int rc = check_attn(kv, r->n_new, r->n_heads, &max_len)) return rc;
+  if (!float_type(r->dtype)) return nrc_fail_api(NRC_ERR_INVALID, "type %d", r->dtype);
+  if (!isfinite(r->scale)) return nrc_fail_api(NRC_ERR_INVALID, "scale is not finite");
+  if (r->weights && (r->weights_len == 0 || r->weights_len > 0x7fffffff))
+    return nrc_fail_api(NRC_ERR_INVALID, "weights of length %llu", (unsigned long long)r->weights_len);
   if (kv->n_seqs == 0) return NRC_OK;
-  if (!out || !q || !lens) return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
-  if (!aligned(out, dtype) || !aligned(q, dtype) || !aligned4(lens, weights))
+  if (!r->out || !r->q || !r->lens) return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if (!aligned(r->out, r->dtype) || !aligned(r->q, r->dtype) || !aligned4(r->lens, r->weights))
     return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
-  const size_t need = paged_attn_workspace(*kv, (uint32_t)n_new, (uint32_t)n_heads, weights != nullptr, (uint32_t)max_len);
-  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return nrc_fail_api(NRC_ERR_INVALID, "workspace of %zu bytes, 16-byte aligned: %zu needed",
-                        workspace ? workspace_bytes : 0, need);
   PagedAttnArgs a{};
   a.kv = *kv;
-  a.out = out;
-  a.q = q;
-  a.o_seq = o_seq, a.o_token = o_token, a.o_head = o_head;
-  a.q_seq = q_seq, a.q_token = q_token, a.q_head = q_head;
-  a.dtype = dtype;
-  a.n_new = (uint32_t)n_new, a.n_heads = (uint32_t)n_heads, a.max_len = (uint32_t)max_len;
-  a.lens = lens;
-  a.scale = scale;
-  a.weights = weights;
-  a.weights_len = (uint32_t)weights_len;
-  a.workspace = workspace;
+  a.out = r->out;
+  a.q = r->q;
+  a.o_seq = r->o_seq, a.o_token = r->o_token, a.o_head = r->o_head;
+  a.q_seq = r->q_seq, a.q_token = r->q_token, a.q_head = r->q_head;
+  a.dtype = r->dtype;
+  a.n_new = (uint32_t)r->n_new, a.n_heads = (uint32_t)r->n_heads, a.max_len = (uint32_t)max_len;
+  a.lens = r->lens;
+  a.scale = r->scale;
+  a.weights = r->weights;
+  a.weights_len = (uint32_t)r->weights_len;
+  a.workspace = r->workspace;
+  const size_t need = paged_attn_workspace(*kv, a.n_new, a.n_heads, a.weights != nullptr, a.max_len);
+  if (need && (!r->workspace || r->workspace_bytes < need || !aligned16(r->workspace)))
+    return nrc_fail_api(NRC_ERR_INVALID, "workspace of %llu bytes, 16-byte aligned: %zu needed",
+                        r->workspace ? (unsigned long long)r->workspace_bytes : 0ull, need);
   return cuda_rc(paged_attn_run(a, static_cast<cudaStream_t>(stream)), "attn_paged");
 }
 

@@ -1,4 +1,6 @@
 // Host side of the paged attention: the variant, the schedule and the workspace's layout.
+#include <atomic>
+
 #include "paged_attn.cuh"
 
 namespace nrc {
@@ -8,11 +10,32 @@ __device__ unsigned g_attn_err;
 
 using pattn::Plan;
 
+// SM count and error word of the current device, looked up once per device (no lock: each slot is written with the same
+// values by whoever comes first).
+struct Device {
+  std::atomic<int> sms{0};
+  std::atomic<unsigned*> err{nullptr};
+};
+constexpr int MAX_DEVICES = 64;
+Device g_devices[MAX_DEVICES];
+
 int sm_count() {
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;  // only a size asked for without a device
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= MAX_DEVICES) return 148;  // only a size asked for without a device
+  if ((n = g_devices[dev].sms.load(std::memory_order_relaxed))) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  g_devices[dev].sms.store(n, std::memory_order_relaxed);
   return n;
+}
+cudaError_t error_word(unsigned** err) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < MAX_DEVICES && (*err = g_devices[dev].err.load(std::memory_order_relaxed))) return cudaSuccess;
+  void* p = nullptr;
+  if (cudaError_t e = cudaGetSymbolAddress(&p, g_attn_err)) return e;
+  *err = static_cast<unsigned*>(p);
+  if (dev < MAX_DEVICES) g_devices[dev].err.store(*err, std::memory_order_relaxed);
+  return cudaSuccess;
 }
 
 // Parts of the cache's type that hold the bits of q's (and out's) type.
@@ -79,9 +102,7 @@ cudaError_t paged_attn_run(const PagedAttnArgs& a, cudaStream_t s) {
   p.a = a;
   int nt;
   make_plan(p, &nt, static_cast<uint8_t*>(a.workspace));
-  void* err = nullptr;
-  if (cudaError_t e = cudaGetSymbolAddress(&err, g_attn_err)) return e;
-  p.err = static_cast<unsigned*>(err);
+  if (cudaError_t e = error_word(&p.err)) return e;
   const int parts = parts_of(a.kv.dtype, a.dtype);
   if (a.kv.dtype == NRC_F16) return parts == 2 ? paged_attn_f16_2(p, nt, s) : paged_attn_f16_1(p, nt, s);
   return parts == 3 ? paged_attn_bf16_3(p, nt, s) : parts == 2 ? paged_attn_bf16_2(p, nt, s) : paged_attn_bf16_1(p, nt, s);

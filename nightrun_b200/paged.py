@@ -8,12 +8,17 @@ made on theirs. Shapes, types, strides and devices that do not fit raise
 NrcError (INVALID); tensors that are not on a GPU raise ValueError.
 """
 import ctypes as C
+import struct
 
 import torch
 
 from ._lib import NRC_ERR_INVALID, NrcError, PagedKVDesc, check, lib
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_I32 = torch.int32
+# nrc_rope_args and nrc_attn_args, packed in one step: a ctypes structure takes three times as long to fill.
+_ROPE_ARGS = struct.Struct("QqqQqqQqqQqqQQQQQQQiif4x")
+_ATTN_ARGS = struct.Struct("QqqqQqqqQQQQQQQQif")
 
 
 def _need(ok, what):
@@ -28,16 +33,16 @@ def _type(t):
     return d
 
 
-def _on(device, *tensors):
+def _elsewhere(device, *tensors):
+    """Raises for the tensor that is not on `device`."""
     for t in tensors:
-        if t.device != device:
-            if not t.is_cuda:
-                raise ValueError("nrcuda kernels take CUDA tensors")
-            raise NrcError(NRC_ERR_INVALID, f"tensors on {device} and {t.device}")
+        if not t.is_cuda:
+            raise ValueError("nrcuda kernels take CUDA tensors")
+        _need(t.device == device, f"tensors on {device} and {t.device}")
 
 
 def _ints(t, shape, what):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or not t.is_contiguous():
         raise NrcError(NRC_ERR_INVALID, f"{what}: contiguous int32 of shape {tuple(shape)}")
 
 
@@ -48,7 +53,7 @@ def _call(device, stream, fn, *args):
         _need(stream.device == device, f"a stream of {stream.device} for tensors on {device}")
         handle = stream.cuda_stream
     else:
-        handle = torch._C._cuda_getCurrentRawStream(index)
+        handle = torch._C._cuda_getCurrentRawStream(index)  # current_stream() takes 3 us to wrap it
     if torch.cuda.current_device() == index:
         rc = fn(*args, handle)
     else:
@@ -68,7 +73,7 @@ class PagedKV:
     def __init__(self, k_pages, v_pages, table):
         if not (k_pages.is_cuda and v_pages.is_cuda and table.is_cuda):
             raise ValueError("nrcuda kernels take CUDA tensors")
-        _on(k_pages.device, v_pages, table)
+        _elsewhere(k_pages.device, v_pages, table)
         _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride()
               and k_pages.dtype == v_pages.dtype, "k_pages and v_pages: two alike [pages, page size, KV heads, head dim]")
         _need(k_pages.dtype in (torch.float16, torch.bfloat16), "pages are float16 or bfloat16")
@@ -77,7 +82,7 @@ class PagedKV:
         _need(table.dtype == torch.int32 and table.dim() == 2 and (table.stride(1) == 1 or table.shape[1] < 2),
               "table: int32 [sequences, pages], rows contiguous")
         self.k_pages, self.v_pages, self.table = k_pages, v_pages, table
-        self.device = k_pages.device
+        self.device, self.index = k_pages.device, k_pages.device.index
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k_pages.shape
         self.n_seqs, self.max_pages = table.shape
         ps, rs, hs, _ = k_pages.stride()
@@ -90,14 +95,6 @@ class PagedKV:
                                 self.page_size, self.n_kv_heads, self.head_dim, self.n_seqs, self.max_pages,
                                 table.stride(0) if self.n_seqs > 1 else self.max_pages, _DTYPES[k_pages.dtype])
         self._ref = C.byref(self.desc)
-
-
-def _heads(t, lead, kv, what):
-    """Strides of [*lead, heads, head_dim], the last dimension contiguous."""
-    s = t.stride()
-    if t.dim() != lead + 2 or t.shape[-1] != kv.head_dim or s[-1] != 1:
-        raise NrcError(NRC_ERR_INVALID, f"{what}: [..., heads, {kv.head_dim}] with a contiguous head dimension")
-    return s
 
 
 def rope_freqs_yarn(rot_dim, theta, factor, original_context, beta_fast=32.0, beta_slow=1.0):
@@ -114,33 +111,35 @@ def rope_append(q_out, q, k, v, kv, freqs, pos, seq, slot, style=1, mscale=1.0, 
     cached). freqs: float32 CUDA tensor, one value per rotated pair (the head's first 2 * numel
     values turn); pos, seq, slot: int32 [tokens]; style 0 = Adjacent, 1 = Neox. No two tokens of a
     call share (seq, slot)."""
-    dev, dt = kv.device, _type(q)
-    _on(dev, q_out, q, k, v, freqs, pos, seq, slot)
-    n = (q.shape[0],)
-    qs, ks, vs, os_ = _heads(q, 1, kv, "q"), _heads(k, 1, kv, "k"), _heads(v, 1, kv, "v"), _heads(q_out, 1, kv, "q_out")
-    if q_out.shape != q.shape or k.shape != v.shape or k.shape[0] != n[0] or k.shape[1] != kv.n_kv_heads or not (
-            k.dtype == v.dtype == q_out.dtype == q.dtype):
-        raise NrcError(NRC_ERR_INVALID, "q, q_out [tokens, heads, head_dim] and k, v [tokens, KV heads, head_dim] of one type")
-    _need(freqs.dtype == torch.float32 and freqs.dim() == 1 and freqs.is_contiguous(), "freqs: contiguous float32")
-    _ints(pos, n, "pos"), _ints(seq, n, "seq"), _ints(slot, n, "slot")
-    _call(dev, stream, lib().nrc_rope_append, kv._ref, q_out.data_ptr(), os_[0], os_[1], q.data_ptr(), qs[0], qs[1],
-          k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, n[0], q.shape[1], freqs.data_ptr(),
-          2 * freqs.numel(), mscale, style, pos.data_ptr(), seq.data_ptr(), slot.data_ptr())
-
-
-def _attn_shape(q, kv):
-    """q [seqs, new, heads, head_dim], or [seqs, heads, head_dim] for one new token each."""
-    if q.dim() == 3:
-        q = q.unsqueeze(1)
-    _heads(q, 2, kv, "q")
-    return q
+    i = kv.index
+    if not (q.get_device() == i == k.get_device() == v.get_device() == q_out.get_device() == freqs.get_device()
+            == pos.get_device() == seq.get_device() == slot.get_device()):
+        _elsewhere(kv.device, q_out, q, k, v, freqs, pos, seq, slot)
+    qz, kz, dt, d = q.shape, k.shape, q.dtype, kv.head_dim
+    if (len(qz) != 3 or q_out.shape != qz or qz[2] != d or kz != (qz[0], kv.n_kv_heads, d) or v.shape != kz
+            or k.dtype is not dt or v.dtype is not dt or q_out.dtype is not dt):
+        raise NrcError(NRC_ERR_INVALID, f"q, q_out [tokens, heads, {d}] and k, v [tokens, {kv.n_kv_heads}, {d}] of one type")
+    (qt, qh, a), (kt, kh, b), (vt, vh, c), (ot, oh, e) = q.stride(), k.stride(), v.stride(), q_out.stride()
+    if not a == b == c == e == 1:
+        raise NrcError(NRC_ERR_INVALID, "the head dimension is contiguous")
+    if freqs.dtype is not torch.float32 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise NrcError(NRC_ERR_INVALID, "freqs: contiguous float32")
+    n = qz[:1]
+    if (pos.dtype is not _I32 or seq.dtype is not _I32 or slot.dtype is not _I32 or not pos.shape == seq.shape == slot.shape == n
+            or not (pos.is_contiguous() and seq.is_contiguous() and slot.is_contiguous())):
+        raise NrcError(NRC_ERR_INVALID, "pos, seq, slot: contiguous int32 [tokens]")
+    _call(kv.device, stream, lib().nrc_rope_append, kv._ref, _ROPE_ARGS.pack(
+        q_out.data_ptr(), ot, oh, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, freqs.data_ptr(),
+        pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n[0], qz[1], 2 * freqs.numel(),
+        _DTYPES[dt] if dt in _DTYPES else _type(q), style, mscale))
 
 
 def attn_paged_workspace(q, kv, weights=False, max_len=0):
     """The workspace of attn_paged calls of this shape: keep it, and use it in one call at a time."""
-    q = _attn_shape(q, kv)
+    _need(q.dim() in (3, 4), "q: [seqs, new, heads, head_dim] or [seqs, heads, head_dim]")
     need = C.c_size_t()
-    check(lib().nrc_attn_paged_workspace(kv._ref, q.shape[1], q.shape[2], int(weights), max_len, C.byref(need)))
+    check(lib().nrc_attn_paged_workspace(kv._ref, q.shape[1] if q.dim() == 4 else 1, q.shape[-2], int(weights), max_len,
+                                         C.byref(need)))
     return torch.empty(need.value, dtype=torch.uint8, device=kv.device)
 
 
@@ -151,20 +150,33 @@ def attn_paged(out, q, kv, lens, scale, weights=None, max_len=0, workspace=None,
     that sees nothing gets zeros. weights (float32 [seqs, KV heads, slots]): what every position
     received is added to it. max_len: no sequence is longer (0: the table's width). Without a
     workspace one is allocated for the call."""
-    dev, dt = kv.device, _type(q)
-    _on(dev, out, q, lens)
-    if out.shape != q.shape or out.dtype != q.dtype:
+    i = kv.index
+    if not q.get_device() == i == out.get_device() == lens.get_device():
+        _elsewhere(kv.device, out, q, lens)
+    z, dt, n = q.shape, q.dtype, kv.n_seqs
+    if out.shape != z or out.dtype is not dt:
         raise NrcError(NRC_ERR_INVALID, "out is like q")
-    q, o = _attn_shape(q, kv), _attn_shape(out, kv)
-    n, new, heads, _ = q.shape
-    _need(n == kv.n_seqs, "q, lens and the table hold the same sequences")
+    if len(z) == 4:
+        _, new, heads, d = z
+        (qs, qt, qh, a), (os_, ot, oh, b) = q.stride(), out.stride()
+    elif len(z) == 3:
+        new, (_, heads, d) = 1, z
+        (qs, qh, a), (os_, oh, b) = q.stride(), out.stride()
+        qt = ot = 0
+    else:
+        raise NrcError(NRC_ERR_INVALID, "q: [seqs, new, heads, head_dim] or [seqs, heads, head_dim]")
+    if z[0] != n or d != kv.head_dim or not a == b == 1:
+        raise NrcError(NRC_ERR_INVALID, f"q: [{n} sequences as in the table, ..., heads, {kv.head_dim}], the last contiguous")
     _ints(lens, (n,), "lens")
-    wp, wl = None, 0
+    wp = wl = 0
     if weights is not None:
-        _on(dev, weights)
-        _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.is_contiguous()
-              and weights.shape[:2] == (n, kv.n_kv_heads), "weights: contiguous float32 [seqs, KV heads, slots]")
+        if weights.get_device() != i:
+            _elsewhere(kv.device, weights)
+        if (weights.dtype is not torch.float32 or weights.dim() != 3 or not weights.is_contiguous()
+                or weights.shape[:2] != (n, kv.n_kv_heads)):
+            raise NrcError(NRC_ERR_INVALID, "weights: contiguous float32 [seqs, KV heads, slots]")
         wp, wl = weights.data_ptr(), weights.shape[2]
+    _need(max_len >= 0, "negative max_len")
     if workspace is None:
         if stream is None:
             workspace = attn_paged_workspace(q, kv, weights is not None, max_len)
@@ -172,11 +184,13 @@ def attn_paged(out, q, kv, lens, scale, weights=None, max_len=0, workspace=None,
             with torch.cuda.stream(stream):  # the allocator hands it out again behind this call
                 workspace = attn_paged_workspace(q, kv, weights is not None, max_len)
     else:
-        _on(dev, workspace)
-        _need(workspace.is_contiguous(), "the workspace is contiguous")
-    qs, os_ = q.stride(), o.stride()
-    _call(dev, stream, lib().nrc_attn_paged, kv._ref, o.data_ptr(), os_[0], os_[1], os_[2], q.data_ptr(), qs[0], qs[1],
-          qs[2], dt, new, heads, lens.data_ptr(), scale, wp, wl, max_len, workspace.data_ptr(), workspace.nbytes)
+        if workspace.get_device() != i:
+            _elsewhere(kv.device, workspace)
+        if not workspace.is_contiguous():
+            raise NrcError(NRC_ERR_INVALID, "the workspace is contiguous")
+    _call(kv.device, stream, lib().nrc_attn_paged, kv._ref, _ATTN_ARGS.pack(
+        out.data_ptr(), os_, ot, oh, q.data_ptr(), qs, qt, qh, lens.data_ptr(), wp, workspace.data_ptr(), workspace.nbytes,
+        wl, max_len, new, heads, _DTYPES[dt] if dt in _DTYPES else _type(q), scale))
 
 
 def evict(kept, new_lens, new_weights, kv, lens, weights, recent, sinks=0, stream=None):
@@ -185,19 +199,22 @@ def evict(kept, new_lens, new_weights, kv, lens, weights, recent, sinks=0, strea
     compacts its pages in place. kept: int32 [seqs, KV heads, budget], the old slots in ascending
     order, -1 behind a shorter sequence's; new_lens int32 [seqs]; weights, new_weights: float32
     [seqs, KV heads, slots]. new_lens may be lens, new_weights may be weights."""
-    dev = kv.device
-    _on(dev, kept, new_lens, new_weights, lens, weights)
-    n = (kv.n_seqs,)
-    _ints(lens, n, "lens"), _ints(new_lens, n, "new_lens")
-    _need(kept.dim() == 3 and kept.shape[:2] == (kv.n_seqs, kv.n_kv_heads), "kept: [seqs, KV heads, budget]")
-    _ints(kept, kept.shape, "kept")
-    for t in (weights, new_weights):
-        if (t.dtype != torch.float32 or t.dim() != 3 or not t.is_contiguous() or t.shape != weights.shape
-                or t.shape[0] != kv.n_seqs or t.shape[1] != kv.n_kv_heads):
-            raise NrcError(NRC_ERR_INVALID, "weights, new_weights: contiguous float32 [seqs, KV heads, slots]")
+    i = kv.index
+    if not (kept.get_device() == i == new_lens.get_device() == new_weights.get_device() == lens.get_device()
+            == weights.get_device()):
+        _elsewhere(kv.device, kept, new_lens, new_weights, lens, weights)
+    n, kz, wz = (kv.n_seqs,), kept.shape, weights.shape
+    _ints(lens, n, "lens")
+    _ints(new_lens, n, "new_lens")
+    if len(kz) != 3 or kz[:2] != (n[0], kv.n_kv_heads):
+        raise NrcError(NRC_ERR_INVALID, "kept: [seqs, KV heads, budget]")
+    _ints(kept, kz, "kept")
+    if (len(wz) != 3 or wz[:2] != kz[:2] or new_weights.shape != wz or weights.dtype is not torch.float32
+            or new_weights.dtype is not torch.float32 or not (weights.is_contiguous() and new_weights.is_contiguous())):
+        raise NrcError(NRC_ERR_INVALID, "weights, new_weights: contiguous float32 [seqs, KV heads, slots]")
     _need(recent >= 0 and sinks >= 0, "negative counts")
-    _call(dev, stream, lib().nrc_kv_evict, kv._ref, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
-          lens.data_ptr(), weights.data_ptr(), weights.shape[2], kept.shape[2], recent, sinks)
+    _call(kv.device, stream, lib().nrc_kv_evict, kv._ref, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
+          lens.data_ptr(), weights.data_ptr(), wz[2], kz[2], recent, sinks)
 
 
 def verify_draft(tokens, accepted, p, q, draft, u, n_draft=None, stream=None):
@@ -206,23 +223,29 @@ def verify_draft(tokens, accepted, p, q, draft, u, n_draft=None, stream=None):
     int32 [seqs] (None: n). Draft i is taken while u[i] * q_i(draft) < p_i(draft); the token after the
     taken ones is drawn with u[n] from max(p - q, 0) at a refusal, else from p. tokens int32
     [seqs, n + 1]: taken drafts, the drawn token, -1; accepted int32 [seqs]: how many were taken."""
-    if not p.is_cuda:
-        raise ValueError("nrcuda kernels take CUDA tensors")
-    dev, dt = p.device, _type(p)
-    _on(dev, tokens, accepted, draft, u)
-    _need(p.dim() == 3 and p.shape[1] > 0 and p.stride(2) == 1, "p: [seqs, n + 1, vocab], rows contiguous")
-    b, m, vocab = p.shape
-    ps, qp, qs = p.stride(), None, (0, 0)
+    i, dt = p.get_device(), p.dtype
+    if i < 0 or not i == tokens.get_device() == accepted.get_device() == draft.get_device() == u.get_device():
+        _elsewhere(p.device, p, tokens, accepted, draft, u)
+    z = p.shape
+    _need(len(z) == 3 and z[1] > 0, "p: [seqs, n + 1, vocab]")
+    b, m, vocab = z
+    (ps, pt, one), qp, qs, qt = p.stride(), 0, 0, 0
     if q is not None:
-        _on(dev, q)
-        _need(q.dtype == p.dtype and q.shape == (b, m - 1, vocab) and q.stride(2) == 1,
-              "q: [seqs, n, vocab] of p's type, rows contiguous")
-        qp, qs = q.data_ptr(), q.stride()
-    _ints(tokens, (b, m), "tokens"), _ints(accepted, (b,), "accepted"), _ints(draft, (b, m - 1), "draft")
-    _need(u.dtype == torch.float32 and u.shape == (b, m) and u.is_contiguous(), "u: contiguous float32 [seqs, n + 1]")
+        if q.get_device() != i:
+            _elsewhere(p.device, q)
+        _need(q.dtype is dt and q.shape == (b, m - 1, vocab), "q: [seqs, n, vocab] of p's type")
+        qp, (qs, qt, two) = q.data_ptr(), q.stride()
+        one = one if two == 1 else two
+    _need(one == 1 or vocab == 1, "the rows of p and q are contiguous")
+    _ints(tokens, (b, m), "tokens")
+    _ints(accepted, (b,), "accepted")
+    _ints(draft, (b, m - 1), "draft")
+    if u.dtype is not torch.float32 or u.shape != (b, m) or not u.is_contiguous():
+        raise NrcError(NRC_ERR_INVALID, "u: contiguous float32 [seqs, n + 1]")
     if n_draft is not None:
-        _on(dev, n_draft)
+        if n_draft.get_device() != i:
+            _elsewhere(p.device, n_draft)
         _ints(n_draft, (b,), "n_draft")
-    _call(dev, stream, lib().nrc_verify_draft, tokens.data_ptr(), accepted.data_ptr(), p.data_ptr(), ps[0], ps[1], qp,
-          qs[0], qs[1], dt, b, m - 1, vocab, draft.data_ptr(), u.data_ptr(),
+    _call(p.device, stream, lib().nrc_verify_draft, tokens.data_ptr(), accepted.data_ptr(), p.data_ptr(), ps, pt, qp, qs, qt,
+          _DTYPES[dt] if dt in _DTYPES else _type(p), b, m - 1, vocab, draft.data_ptr(), u.data_ptr(),
           None if n_draft is None else n_draft.data_ptr())

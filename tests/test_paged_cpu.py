@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from nightrun_b200 import _lib, kernels
+from nightrun_b200 import _lib, kernels, paged
 from nightrun_b200._lib import NrcError, PagedKVDesc
 
 FAKE = 0x10000  # never read: every call below is refused before a launch
@@ -31,13 +31,15 @@ BAD_CACHES = [dict(dtype=0), dict(dtype=7), dict(head_dim=48), dict(head_dim=160
 
 
 def rope(L, kv, dtype=0, tokens=4, heads=4, rot=64, style=1, q=FAKE, freqs=FAKE, pos=FAKE):
-    return L.nrc_rope_append(kv, FAKE, 256, 64, q, 256, 64, FAKE, 128, 64, FAKE, 128, 64, dtype, tokens, heads, freqs, rot,
-                             1.0, style, pos, FAKE, FAKE, None)
+    args = paged._ROPE_ARGS.pack(FAKE, 256, 64, q or 0, 256, 64, FAKE, 128, 64, FAKE, 128, 64, freqs or 0, pos or 0, FAKE,
+                                 FAKE, tokens, heads, rot, dtype, style, 1.0)
+    return L.nrc_rope_append(kv, args, None)
 
 
 def attn(L, kv, dtype=0, new=1, heads=4, scale=0.125, weights=None, wlen=0, ws=None, wsb=0, q=FAKE, lens=FAKE):
-    return L.nrc_attn_paged(kv, FAKE, 256, 256, 64, q, 256, 256, 64, dtype, new, heads, lens, scale, weights, wlen, 0, ws,
-                            wsb, None)
+    args = paged._ATTN_ARGS.pack(FAKE, 256, 256, 64, q or 0, 256, 256, 64, lens or 0, weights or 0, ws or 0, wsb, wlen, 0,
+                                 new, heads, dtype, scale)
+    return L.nrc_attn_paged(kv, args, None)
 
 
 def evict(L, kv, wlen=32, budget=8, recent=2, sinks=1, kept=FAKE, weights=FAKE):
@@ -61,6 +63,7 @@ def test_rope_append_refusals(L):
                dict(pos=FAKE + 1), dict(freqs=FAKE + 2)):
         assert rope(L, desc(), **kw) == -1, kw
         assert L.nrc_last_error()
+    assert L.nrc_rope_append(desc(), None, None) == -1
     assert rope(L, desc(), tokens=0) == 0  # nothing to do, nothing launched
 
 
@@ -76,6 +79,7 @@ def test_attn_paged_refusals(L):
         assert attn(L, desc(), ws=FAKE, wsb=need.value - 1) == -1
         assert attn(L, desc(), ws=FAKE + 4, wsb=need.value) == -1
         assert attn(L, desc(), ws=None, wsb=need.value) == -1
+    assert L.nrc_attn_paged(desc(), None, None) == -1
     assert L.nrc_attn_paged_workspace(desc(), 1, 4, 0, 0, None) == -1
     assert L.nrc_attn_paged_workspace(desc(), 1, 5, 0, 0, C.byref(need)) == -1
     assert attn(L, desc(n_seqs=0), ws=FAKE, wsb=1 << 40) == 0
