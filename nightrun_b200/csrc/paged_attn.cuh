@@ -132,6 +132,9 @@ NRC_DEV uint32_t seq_len(const Plan& p, uint32_t b) {
 }
 // Units of a sequence; an empty one has a unit too, whose block writes its zeros.
 NRC_DEV uint32_t units_of(uint32_t len) { return len ? (len + UNIT - 1) / UNIT : 1u; }
+// What a (sequence, KV head, row block) costs its first block beside its units: the queries, the first tiles' latency, the
+// join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle.
+constexpr uint32_t SETUP = 2;
 
 // K pieces of a tile: [chunk of 32 values][position g or g + 8].
 template <int HD>
@@ -362,7 +365,7 @@ NRC_DEV void scores(float (&s)[NT][4], const KTile<HD>& k, const Queries<HD, PAR
 // Where block `i` starts, and the units each block takes: sequences in order, in each the (KV head, row
 // block) pairs in order (hbs of them), in each its units. Every block finds its start alone, from the lengths.
 struct Start {
-  uint32_t b, hb, unit;  // sequence, pair, first unit
+  uint32_t b, hb, unit;  // sequence, pair, first unit (SETUP units that are no work come first)
   uint64_t left;         // units of work of this block
   uint64_t share, total;
 };
@@ -371,7 +374,7 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start
   const uint32_t per = (n + THREADS - 1) / THREADS, b0 = min(threadIdx.x * per, n), b1 = min(b0 + per, n);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t sum = 0;
-  for (uint32_t b = b0; b < b1; b++) sum += units_of(seq_len(p, b));
+  for (uint32_t b = b0; b < b1; b++) sum += SETUP + units_of(seq_len(p, b));
   uint64_t x = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -393,10 +396,10 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start
   __syncthreads();
   if (start < total && start >= before * hbs && start < (before + sum) * hbs) {
     uint64_t at = start - before * hbs;
-    uint32_t b = b0, u = units_of(seq_len(p, b));
+    uint32_t b = b0, u = SETUP + units_of(seq_len(p, b));
     while (at >= (uint64_t)u * hbs) {
       at -= (uint64_t)u * hbs;
-      u = units_of(seq_len(p, ++b));
+      u = SETUP + units_of(seq_len(p, ++b));
     }
     found->b = b;
     found->hb = (uint32_t)(at / u);
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
     st.b = blockIdx.x / hbs;
     st.hb = blockIdx.x % hbs;
     st.unit = 0;
-    st.left = units_of(seq_len(p, st.b));
+    st.left = SETUP + units_of(seq_len(p, st.b));
     st.share = st.left;
   } else {
     st = find_start(p, hbs, warp_sums, &start_s);
@@ -457,8 +460,10 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
   bool first = true;
   while (st.left) {
     const uint32_t b = st.b, h = st.hb / p.row_blocks, rb = st.hb % p.row_blocks;
-    const uint32_t len = seq_len(p, b), units = units_of(len), u0 = st.unit;
-    const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + st.left);
+    const uint32_t len = seq_len(p, b), units = units_of(len);
+    const uint32_t v0 = st.unit, v1 = (uint32_t)min((uint64_t)(SETUP + units), v0 + st.left);
+    const uint32_t u0 = v0 > SETUP ? v0 - SETUP : 0, u1 = v1 > SETUP ? v1 - SETUP : 0;
+    if (u1 == 0) break;  // the share ends before the first unit: the next block's work
     __syncthreads();  // the queries and sums of the work before are read
     const uint32_t end = min(u1 * UNIT, len);
     Walk walk;
@@ -633,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
       p.cut[blockIdx.x] = make_int4((int)b, (int)st.hb, (int)(1 + (rest + st.share - 1) / st.share), 0);
     }
     first = false;
-    st.left -= u1 - u0;
+    st.left -= v1 - v0;
     st.unit = 0;
     if (++st.hb == hbs) {
       st.hb = 0;
@@ -694,8 +699,10 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
   Start st = find_start(p, hbs, warp_sums, &start_s);
   bool waited = false;
   while (st.left) {
-    const uint32_t b = st.b, h = st.hb, len = seq_len(p, b), units = units_of(len), u0 = st.unit;
-    const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + st.left), end = min(u1 * UNIT, len);
+    const uint32_t b = st.b, h = st.hb, len = seq_len(p, b), units = units_of(len);
+    const uint32_t v0 = st.unit, v1 = (uint32_t)min((uint64_t)(SETUP + units), v0 + st.left);
+    const uint32_t u0 = v0 > SETUP ? v0 - SETUP : 0, u1 = v1 > SETUP ? v1 - SETUP : 0, end = min(u1 * UNIT, len);
+    if (u1 == 0) break;
     float* w = p.a.weights + ((size_t)b * p.a.kv.n_kv_heads + h) * p.a.weights_len;
     const uint32_t all_see = len > p.a.n_new - 1 ? len - (p.a.n_new - 1) : 0;
     for (uint32_t rb = 0; rb < p.row_blocks; rb++) {
@@ -748,7 +755,7 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
         }
       }
     }
-    st.left -= u1 - u0;
+    st.left -= v1 - v0;
     st.unit = 0;
     if (++st.hb == hbs) {
       st.hb = 0;
