@@ -359,7 +359,9 @@ int nrc_sync_check(void* stream) {
   }
   if (paged | attn)
     return nrc_fail_api(NRC_ERR_DEVICE, "%s (error bits 0x%x)",
-                        (paged | attn) & ERR_BAD_PAGE ? "a page id outside the pool" : "a length, sequence or slot outside the table",
+                        (paged | attn) & ERR_BAD_PAGE   ? "a page id outside the pool"
+                        : (paged | attn) & ERR_BAD_SLOT ? "a length, sequence or slot outside the table"
+                                                        : "kernel wait expired",
                         paged | attn);
   return NRC_OK;
 }

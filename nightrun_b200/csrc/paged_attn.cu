@@ -44,19 +44,50 @@ int parts_of(int cache, int dtype) {
   return dtype == NRC_F32 ? 3 : dtype == NRC_F16 ? 2 : 1;
 }
 
+// Positions per copy: the largest piece of a page that fills a tile of 128 to 7 parts in 8, in whole groups of 8 rows (the
+// swizzle's). 16 copies per tile at most.
+bool tc_shape(uint32_t page, uint32_t* rows) {
+  for (uint32_t r = pattn::TC_TILE; r >= 8; r -= 8)
+    if (page % r == 0 && pattn::TC_TILE / r * r >= 112) {
+      *rows = r;
+      return true;
+    }
+  return false;
+}
+
+// The tensor maps of the tcgen05 kernel; false where the pages' strides cannot be told to the TMA unit.
+bool make_maps(Plan& p) {
+  const nrc_paged_kv& kv = p.a.kv;
+  auto encode = tensor_map_encoder();
+  if (!encode || kv.pos_stride <= 0 || kv.head_stride <= 0 || kv.page_stride <= 0) return false;
+  const cuuint64_t dims[4] = {kv.head_dim, kv.page_size, kv.n_kv_heads, kv.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.pos_stride * 2, (cuuint64_t)kv.head_stride * 2, (cuuint64_t)kv.page_stride * 2};
+  const cuuint32_t box[4] = {64, p.tc_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const auto type = kv.dtype == NRC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int i = 0; i < 2; i++)
+    if (encode(i ? &p.v_map : &p.k_map, type, 4, i ? kv.v : kv.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  return true;
+}
+
 // Fills the plan and returns the workspace's bytes; `base` null: sizes only.
 size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   const nrc_paged_kv& kv = p.a.kv;
   p.gqa = p.a.n_heads / kv.n_kv_heads;
   p.rows = p.gqa * p.a.n_new;
-  *nt = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
+  const uint32_t units = (p.a.max_len + pattn::UNIT - 1) / pattn::UNIT;
+  p.min_units = 4;
+  // 9 rows and more on the tcgen05 kernel, where its tiles fit: 64 or 128 wide heads, a tail of 15 positions at most, pages
+  // that whole 8-row groups fill.
+  p.tc = p.rows > 8 && p.a.n_new <= 16 && kv.head_dim % 64 == 0 && units > p.min_units && tc_shape(kv.page_size, &p.tc_rows);
+  if (p.tc) p.tc_tile = pattn::TC_TILE / p.tc_rows * p.tc_rows;
+  *nt = p.tc ? 4 : p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
   const uint32_t cols = 8 * *nt;
   p.row_blocks = (p.rows + cols - 1) / cols;
   const uint64_t items = (uint64_t)kv.n_seqs * kv.n_kv_heads * p.row_blocks;
-  const uint32_t units = (p.a.max_len + pattn::UNIT - 1) / pattn::UNIT;
   p.step_pages = pattn::UNIT / kv.page_size;
   p.step_off = pattn::UNIT % kv.page_size;
-  p.min_units = 4;
   p.direct = units <= p.min_units && items <= 0x7fffffffu;
   const uint64_t w_units = (uint64_t)kv.n_seqs * kv.n_kv_heads * (units ? units : 1);
   const uint64_t w_resident = (uint64_t)sm_count() * pattn::WEIGHTS_RESIDENT;
@@ -64,7 +95,7 @@ size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   if (p.direct) {
     p.blocks = (uint32_t)items;
   } else {
-    const uint64_t all = items * units, resident = (uint64_t)sm_count() * pattn::resident(kv.head_dim, *nt);
+    const uint64_t all = items * units, resident = (uint64_t)sm_count() * (p.tc ? 1 : pattn::resident(kv.head_dim, *nt));
     const uint64_t want = (all + p.min_units - 1) / p.min_units;
     p.blocks = (uint32_t)(want < resident ? want : resident);
   }
@@ -102,6 +133,8 @@ cudaError_t paged_attn_run(const PagedAttnArgs& a, cudaStream_t s) {
   p.a = a;
   int nt;
   make_plan(p, &nt, static_cast<uint8_t*>(a.workspace));
+  // Without tensor maps the other kernel runs on the same plan (32 rows at a time, the blocks of this one).
+  if (p.tc && !make_maps(p)) p.tc = 0;
   if (cudaError_t e = error_word(&p.err)) return e;
   const int parts = parts_of(a.kv.dtype, a.dtype);
   if (a.kv.dtype == NRC_F16) return parts == 2 ? paged_attn_f16_2(p, nt, s) : paged_attn_f16_1(p, nt, s);

@@ -1,6 +1,7 @@
 // Attention of the newest tokens of many sequences over a paged KV cache:
-// the kernels, instantiated per cache type by paged_attn_f16.cu and
-// paged_attn_bf16.cu and launched by paged_attn.cu.
+// the kernels for up to 8 query rows per KV head (and for shapes that
+// paged_attn_tc.cuh does not take), instantiated per cache type and number of
+// parts by paged_attn_*_*.cu and launched by paged_attn.cu.
 //
 // Mathematics. For query row r (head r % gqa of the KV head's group, new token r / gqa) over the
 // cached positions t: s_t = f_r (q_r . K_t) with f_r = scale log2(e), m = max s_t, and
@@ -8,8 +9,8 @@
 // taken in one pass with the running maximum, sum and accumulators (all f32) rescaled when the
 // maximum grows, and joined across warps and blocks by the same rule.
 //
-// What bounds it: every K and V row is read once and serves 2 FLOPs per query row and value; with up to 32 rows
-// that is far below the ratio of tensor to memory rate, so the kernel has to keep HBM busy.
+// What bounds it: every K and V row is read once and serves 2 FLOPs per query row and value; that is far below the ratio
+// of tensor to memory rate, so the kernel has to keep HBM busy.
 //
 // Layout. Both products run transposed, with the cache as the 16-row operand A of mma.m16n8k16 and the query rows as
 // its 8 columns: S^T = K Q^T (16 positions x 8 rows) and O^T += V^T P^T (16 values x 8 rows), so that 1..8 rows waste
@@ -25,7 +26,9 @@
 // pieces of the next tile are loaded into the registers of the one before as soon as those are used, 8 KB (of
 // 128-wide f16 heads) per warp in flight. (Pieces copied ahead into shared memory, 190 KB per SM in flight, were
 // slower: 248 against 199 us for 983 MB. It is the warps' instructions per tile that count, not the bytes in
-// flight.) tcgen05 would need 64 or more rows of queries to be fed; its rate is not what is missing.
+// flight.) For a few rows the rate of tcgen05 is not what is missing, and its tiles would have to pass through shared
+// memory. Measured: 64 sequences of 4096, 32/8 heads of 128, bf16: 174 us, 6.2 TB/s (0.95 of measured); 64 ragged ones up to
+// 16384: 158 us (0.96); one of 131072: 88 us and the join 8 us more (0.86).
 //
 // Split parts. The tensor cores take operands of the cache's type. q (scaled by a power of two to at most 2 per row) and
 // p enter as PARTS values of that type whose sum holds the bits that the output's type can show: one where the output is
@@ -33,6 +36,7 @@
 // the same f32 accumulators.
 #pragma once
 #include "paged.cuh"
+#include "tma.cuh"
 
 namespace nrc {
 namespace pattn {
@@ -46,10 +50,13 @@ constexpr int resident(int hd, int nt) { return nt > 1 ? 2 : hd <= 32 ? 4 : 3; }
 
 // What one launch needs beside the arguments.
 struct Plan {
+  CUtensorMap k_map, v_map;        // tc: [page][KV head][position][value] of K and V
   PagedAttnArgs a;
   uint32_t gqa, rows, row_blocks;  // query rows per KV head (gqa * n_new), blocks of 8 * NT of them
   uint32_t blocks;                 // blocks of the attention kernel
   uint32_t weight_blocks;          // blocks of the weights' kernel
+  uint32_t tc;                     // many rows: the kernel of paged_attn_tc.cuh
+  uint32_t tc_rows, tc_tile;       // its copies' positions, and its tiles'
   uint32_t direct;                 // one (sequence, KV head, row block) per block: nothing is split
   uint32_t min_units;
   int4* cut;                       // [blocks]: the work that starts in this block and ends in a later one
@@ -131,10 +138,12 @@ NRC_DEV uint32_t seq_len(const Plan& p, uint32_t b) {
   return (uint32_t)raw;
 }
 // Units of a sequence; an empty one has a unit too, whose block writes its zeros.
-NRC_DEV uint32_t units_of(uint32_t len) { return len ? (len + UNIT - 1) / UNIT : 1u; }
+NRC_DEV uint32_t units_of(uint32_t len, uint32_t unit = UNIT) { return len ? (len + unit - 1) / unit : 1u; }
 // What a (sequence, KV head, row block) costs its first block beside its units: the queries, the first tiles' latency, the
-// join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle.
-constexpr uint32_t SETUP = 2;
+// join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle (64
+// ragged sequences: 188 us uncounted, 158 us; the tcgen05 kernel on 24: 106 us at 6, 73 us at 14, 76 us at 20).
+constexpr uint32_t SETUP = 2, TC_SETUP = 14;
+constexpr int TC_TILE = 128;         // rows of a tile of the tcgen05 kernel
 
 // K pieces of a tile: [chunk of 32 values][position g or g + 8].
 template <int HD>
@@ -369,12 +378,13 @@ struct Start {
   uint64_t left;         // units of work of this block
   uint64_t share, total;
 };
-NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start* found) {
+template <int T = THREADS>
+NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint32_t unit, uint32_t setup, uint64_t* warp_sums, Start* found) {
   const uint32_t n = p.a.kv.n_seqs;
-  const uint32_t per = (n + THREADS - 1) / THREADS, b0 = min(threadIdx.x * per, n), b1 = min(b0 + per, n);
+  const uint32_t per = (n + T - 1) / T, b0 = min(threadIdx.x * per, n), b1 = min(b0 + per, n);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t sum = 0;
-  for (uint32_t b = b0; b < b1; b++) sum += SETUP + units_of(seq_len(p, b));
+  for (uint32_t b = b0; b < b1; b++) sum += setup + units_of(seq_len(p, b), unit);
   uint64_t x = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -384,7 +394,7 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   uint64_t before = x - sum, all = 0;
-  for (int w = 0; w < WARPS; w++) {
+  for (int w = 0; w < T / 32; w++) {
     if (w < warp) before += warp_sums[w];
     all += warp_sums[w];
   }
@@ -396,10 +406,10 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint64_t* warp_sums, Start
   __syncthreads();
   if (start < total && start >= before * hbs && start < (before + sum) * hbs) {
     uint64_t at = start - before * hbs;
-    uint32_t b = b0, u = SETUP + units_of(seq_len(p, b));
+    uint32_t b = b0, u = setup + units_of(seq_len(p, b), unit);
     while (at >= (uint64_t)u * hbs) {
       at -= (uint64_t)u * hbs;
-      u = SETUP + units_of(seq_len(p, ++b));
+      u = setup + units_of(seq_len(p, ++b), unit);
     }
     found->b = b;
     found->hb = (uint32_t)(at / u);
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
     st.left = SETUP + units_of(seq_len(p, st.b));
     st.share = st.left;
   } else {
-    st = find_start(p, hbs, warp_sums, &start_s);
+    st = find_start(p, hbs, UNIT, SETUP, warp_sums, &start_s);
     if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   bool first = true;
@@ -696,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
   __shared__ Start start_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t hbs = p.a.kv.n_kv_heads;
-  Start st = find_start(p, hbs, warp_sums, &start_s);
+  Start st = find_start(p, hbs, UNIT, SETUP, warp_sums, &start_s);
   bool waited = false;
   while (st.left) {
     const uint32_t b = st.b, h = st.hb, len = seq_len(p, b), units = units_of(len);
@@ -765,13 +775,25 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
   if (!waited) pdl_wait();
 }
 
+template <bool BF, int HD, int PARTS>
+cudaError_t launch_tc(Plan& p, cudaStream_t s);
+
 template <bool BF, int HD, int PARTS, int NT>
-cudaError_t launch(Plan& p, cudaStream_t s) {
+cudaError_t launch_rows(Plan& p, cudaStream_t s) {
   void* args[] = {&p};
   const void* attn = (const void*)k_attn<BF, HD, PARTS, NT>;
   constexpr int sums = WARPS * 8 * NT * (HD + 2) * 4;
   if (cudaError_t e = ensure_smem_attr(attn, sums)) return e;
-  if (cudaError_t e = launch_kernel(attn, dim3(p.blocks), dim3(THREADS), sums, s, false, args)) return e;
+  return launch_kernel(attn, dim3(p.blocks), dim3(THREADS), sums, s, false, args);
+}
+
+template <bool BF, int HD, int PARTS, int NT>
+cudaError_t launch(Plan& p, cudaStream_t s) {
+  void* args[] = {&p};
+  cudaError_t err = cudaSuccess;
+  if constexpr (NT == 4 && HD % 64 == 0) err = p.tc ? launch_tc<BF, HD, PARTS>(p, s) : launch_rows<BF, HD, PARTS, NT>(p, s);
+  else err = launch_rows<BF, HD, PARTS, NT>(p, s);
+  if (err) return err;
   if (!p.direct) {
     int cols = 8 * NT;
     void* jargs[] = {&p, &cols};

@@ -1,5 +1,5 @@
 // Paged attention over a f16 cache, queries and weights in 1 part(s).
-#include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace nrc {
 cudaError_t paged_attn_f16_1(pattn::Plan& p, int nt, cudaStream_t s) { return pattn::launch_hd<false, 1>(p, nt, s); }

@@ -142,7 +142,15 @@ ATTN = [  # lens, new, heads, kv heads, dim, type, cache, page, weights
     ([63, 64, 65, 129, 255, 256, 257], 1, 3, 3, 32, F32, BF16, 1, True), ([1000, 3], 5, 40, 8, 64, F32, F16, 24, True),
     ([4, 0, 1, 2, 3, 5], 4, 4, 2, 32, F16, BF16, 3, True), ([2000], 8, 6, 2, 128, BF16, F16, 100, True),
     ([3000, 1200, 40], 2, 9, 3, 128, F32, F16, 64, False), ([333], 64, 2, 1, 64, F16, F16, 7, True),
-    ([129] * 9, 1, 16, 1, 128, F32, BF16, 32, True), ([700, 20], 3, 33, 3, 64, BF16, BF16, 48, True)]
+    ([129] * 9, 1, 16, 1, 128, F32, BF16, 32, True), ([700, 20], 3, 33, 3, 64, BF16, BF16, 48, True),
+    # 9 rows and more per KV head over longer tables: the tcgen05 kernel
+    ([600], 3, 8, 2, 64, F16, F16, 16, False), ([128, 129, 127, 700, 1], 4, 12, 4, 128, F16, F16, 64, True),
+    ([1500, 2, 0, 515], 16, 4, 2, 64, F32, F16, 9, True), ([999], 5, 16, 4, 128, F32, BF16, 16, True),
+    ([2100, 300], 2, 20, 2, 64, F16, BF16, 24, False), ([5000, 17, 640], 1, 40, 4, 128, BF16, BF16, 128, True),
+    ([1300], 7, 36, 3, 128, F32, F16, 20, True),
+    ([1111, 500, 64], 3, 8, 2, 64, F32, F16, 8, True), ([2000], 2, 12, 2, 128, F16, F16, 40, True),
+    ([700, 480, 481], 4, 6, 2, 64, BF16, BF16, 160, False), ([900, 256], 3, 14, 2, 128, BF16, BF16, 256, True),
+    ([1200], 6, 4, 2, 64, F16, F16, 56, False)]
 
 
 @pytest.mark.parametrize("lens,new,hq,hk,d,dt,ct,page,weights", ATTN, ids=[str(i) for i in range(len(ATTN))])
@@ -204,15 +212,16 @@ def test_attn_paged_far_scales(K, power):
     check_attn(K, q, k, v, table, lens, kv, out, 0.125 * 2.0 ** -power)
 
 
+@pytest.mark.parametrize("heads", [4, 12])
 @pytest.mark.parametrize("ct,dt", [(F16, F32), (BF16, BF16)])
-def test_attn_paged_steep_scores(K, ct, dt):
+def test_attn_paged_steep_scores(K, ct, dt, heads):
     """Scores hundreds apart: one position takes nearly all of a row, wherever it lies."""
     k, v, table, lens, kv = cache_of(K, [700, 699, 64, 2], 1, 64, 16, ct, 8)
-    q = (torch.randn(4, 1, 4, 64, generator=gen(9)) * 12).to(dt)
+    q = (torch.randn(4, 1, heads, 64, generator=gen(9)) * 12).to(dt)
     for s, t in ((0, 0), (1, 698), (2, 17), (3, 1)):
         R.put(k, table, s, t, (q[s, 0, :1].double() / 2).to(ct))
     kv = cuda_kv(K, k, v, table)
-    out = torch.empty(4, 1, 4, 64, dtype=dt, device="cuda")
+    out = torch.empty(4, 1, heads, 64, dtype=dt, device="cuda")
     K.attn_paged(out, q.cuda(), kv, lens.cuda(), 0.5)
     check_attn(K, q, k, v, table, lens, kv, out, 0.5)
 
@@ -236,6 +245,38 @@ def test_attn_paged_masked_rows_with_infinities(K):
             assert worst(out[:, :3], clean[0][:, :3], tol[:, :3]) <= 1
             if which == 1:  # a value row: the last token's outputs carry it, the weights do not
                 assert not torch.isfinite(out[:, 3]).any() and torch.isfinite(w).all()
+
+
+def test_attn_paged_many_rows_with_infinities(K):
+    """The same on the tcgen05 kernel, the infinite rows at the end of a tile, at its start and in the middle; a bad page."""
+    g = gen(17)
+    k, v, table, lens, _ = cache_of(K, [640, 513, 300], 2, 64, 16, F16, 18)
+    q = torch.randn(3, 4, 12, 64, generator=g)
+    clean = R.attention(q, k, v, table, lens, 0.125)
+    tol, _ = R.attention_tolerance(F32, F16, 64, 640, clean[2], clean[3], clean[0])
+    for value in (float("inf"), NAN):
+        for which in (0, 1):
+            k2, v2 = k.clone(), v.clone()
+            for s in range(3):
+                for back in (1, 2):
+                    R.put((k2, v2)[which], table, s, int(lens[s]) - back, torch.full((2, 64), value).to(F16))
+            kv = cuda_kv(K, k2, v2, table)
+            out = torch.empty(3, 4, 12, 64, device="cuda")
+            K.attn_paged(out, q.cuda(), kv, lens.cuda(), 0.125)
+            assert worst(out[:, :2], clean[0][:, :2], tol[:, :2]) <= 1
+            if which == 1:
+                assert not torch.isfinite(out[:, 2:]).any()
+    broken = table.clone()
+    broken[0, 3] = 10 ** 6
+    out = torch.empty(3, 4, 12, 64, device="cuda")
+    K.attn_paged(out, q.cuda(), cuda_kv(K, k, v, broken), lens.cuda(), 0.125)
+    with pytest.raises(NrcError):
+        K.sync_check()
+    assert worst(out[1:], clean[0][1:], tol[1:]) <= 1
+    keep = [t for t in range(640) if not 48 <= t < 64]
+    kk, vv = (R.rows(x, table, 0, keep).double() for x in (k, v))
+    p = torch.softmax(q[0, 3, 0].double() @ kk[:, 0].T * 0.125, -1)
+    assert torch.allclose(out[0, 3, 0].double().cpu(), p @ vv[:, 0], atol=1e-5)
 
 
 def test_attn_paged_strides_and_shapes(K):
