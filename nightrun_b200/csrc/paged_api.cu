@@ -38,6 +38,8 @@ int check_kv(const nrc_paged_kv* kv) {
   if (kv->table_stride < kv->max_pages) return nrc_fail_api(NRC_ERR_INVALID, "table rows overlap");
   if (kv->n_pages && (!kv->k || !kv->v)) return nrc_fail_api(NRC_ERR_INVALID, "null pages");
   if (kv->n_seqs && kv->max_pages && !kv->table) return nrc_fail_api(NRC_ERR_INVALID, "null table");
+  if ((kv->n_pages > 1 && !kv->page_stride) || (kv->page_size > 1 && !kv->pos_stride) || (kv->n_kv_heads > 1 && !kv->head_stride))
+    return nrc_fail_api(NRC_ERR_INVALID, "rows of the pages overlap");
   if (!aligned4(kv->table)) return nrc_fail_api(NRC_ERR_INVALID, "table is not 4-byte aligned");
   if (!aligned16(kv->k) || !aligned16(kv->v) || kv->page_stride % 8 || kv->pos_stride % 8 || kv->head_stride % 8)
     return nrc_fail_api(NRC_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
@@ -78,6 +80,8 @@ int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* r, void* stream
   if (r->tokens == 0) return NRC_OK;
   if ((r->n_heads && (!r->q_out || !r->q)) || !r->k || !r->v || !r->pos || !r->seq || !r->slot || (r->rot_dim && !r->freqs))
     return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if ((r->tokens > 1 && r->n_heads && !r->qo_token) || (r->n_heads > 1 && !r->qo_head))
+    return nrc_fail_api(NRC_ERR_INVALID, "rows of q_out overlap");
   if (!aligned(r->q, r->dtype) || !aligned(r->k, r->dtype) || !aligned(r->v, r->dtype) || !aligned(r->q_out, r->dtype) ||
       !aligned4(r->freqs, r->pos, r->seq, r->slot))
     return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
@@ -112,6 +116,8 @@ int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* r, void* stream)
     return nrc_fail_api(NRC_ERR_INVALID, "weights of length %llu", (unsigned long long)r->weights_len);
   if (kv->n_seqs == 0) return NRC_OK;
   if (!r->out || !r->q || !r->lens) return nrc_fail_api(NRC_ERR_INVALID, "null pointer");
+  if ((kv->n_seqs > 1 && !r->o_seq) || (r->n_new > 1 && !r->o_token) || (r->n_heads > 1 && !r->o_head))
+    return nrc_fail_api(NRC_ERR_INVALID, "rows of out overlap");
   if (!aligned(r->out, r->dtype) || !aligned(r->q, r->dtype) || !aligned4(r->lens, r->weights))
     return nrc_fail_api(NRC_ERR_INVALID, "a pointer is not aligned to its type");
   PagedAttnArgs a{};

@@ -89,6 +89,7 @@ class PagedKV:
         _need(self.page_size > 0 and self.n_kv_heads > 0, "empty pages")
         _need(not any(x % 8 for x in (ps, rs, hs)) and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0,
               "pages and their strides must be multiples of 16 bytes")
+        _need(not any(n > 1 and x == 0 for n, x in zip(k_pages.shape, k_pages.stride())), "rows of the pages overlap")
         _need(self.n_pages < 2 ** 31 and self.max_pages * self.page_size < 2 ** 31 and self.n_seqs < 65536
               and self.n_kv_heads <= 16384, "cache too large")
         self.desc = PagedKVDesc(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), self.n_pages, ps, rs, hs,

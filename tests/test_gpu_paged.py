@@ -302,6 +302,28 @@ def test_attn_paged_strides_and_shapes(K):
     assert torch.equal(flat, ow[:, 1, :, :d])
 
 
+@pytest.mark.parametrize("heads", [4, 24])
+def test_attn_paged_page_layouts(K, heads):
+    """K and V interleaved in one pool, and pages that lie head by head, for few and for many rows."""
+    g = gen(19)
+    hk, d, page, per = 2, 64, 16, 30
+    table = torch.randperm(64, generator=g)[:60].view(2, per).to(torch.int32)
+    lens = torch.tensor([470, 333], dtype=torch.int32)
+    q = torch.randn(2, 1, heads, d, generator=g)
+    both = torch.randn(64, 2, page, hk, d, generator=g).to(F16)
+    by_head = [torch.randn(64, hk, page, d, generator=g).to(F16) for _ in range(2)]
+    gb = both.cuda()
+    gh = [t.cuda().transpose(1, 2) for t in by_head]
+    for k, v, gk, gv in ((both[:, 0], both[:, 1], gb[:, 0], gb[:, 1]),
+                         (by_head[0].transpose(1, 2), by_head[1].transpose(1, 2), *gh)):
+        kv = K.PagedKV(gk, gv, table.cuda())
+        out = torch.empty(2, 1, heads, d, device="cuda")
+        w = torch.zeros(2, hk, per * page, device="cuda")
+        K.attn_paged(out, q.cuda(), kv, lens.cuda(), 0.125, weights=w)
+        check_attn(K, q, k, v, table, lens, kv, out, 0.125)
+        assert torch.allclose(w.sum(-1).cpu(), torch.full((2, hk), heads / hk), atol=1e-4)
+
+
 def test_attn_paged_errors_are_reported(K):
     k, v, table, lens, kv = cache_of(K, [30, 20], 1, 32, 8, F16, 14)
     q = torch.randn(2, 1, 2, 32, generator=gen(15))
@@ -590,6 +612,57 @@ def test_other_streams(K):
     assert all(torch.equal(x, want) for o in outs for x in o)
 
 
+FIRST_CALL = """
+import torch
+from nightrun_b200 import kernels as K
+torch.manual_seed(1)
+c = dict(device="cuda")
+kp, vp = (torch.randn(40, 16, 2, 64, **c).half() for _ in range(2))
+kv = K.PagedKV(kp, vp, torch.randperm(40, **c).view(2, 20).int())
+freqs = torch.tensor(K.rope_freqs(64, 10000.0), **c)
+i = torch.arange(2, dtype=torch.int32, **c)
+lens = torch.tensor([300, 211], dtype=torch.int32, **c)
+x = torch.randn(2, 8, 64, **c)
+few, many = torch.randn(2, 1, 4, 64, **c), torch.randn(2, 3, 8, 64, **c)
+o1, o2 = torch.empty_like(few), torch.empty_like(many)
+w = torch.rand(2, 2, 320, **c)
+kept, nl, nw = torch.empty(2, 2, 100, dtype=torch.int32, **c), torch.empty_like(lens), torch.empty_like(w)
+p, q = torch.rand(2, 4, 5000, **c), torch.rand(2, 3, 5000, **c)
+draft, u = torch.randint(0, 5000, (2, 3), **c).int(), torch.rand(2, 4, **c)
+tokens, accepted = torch.empty(2, 4, dtype=torch.int32, **c), torch.empty(2, dtype=torch.int32, **c)
+def step():
+    K.rope_append(x[:, :4], x[:, :4], x[:, 4:6], x[:, 6:], kv, freqs, i, i, i)
+    K.attn_paged(o1, few, kv, lens, 0.125, weights=w)
+    K.attn_paged(o2, many, kv, lens, 0.125)
+    K.evict(kept, nl, nw, kv, lens, w, 20, 2)
+    K.verify_draft(tokens, accepted, p, q, draft, u)
+state = [t.clone() for t in (x, kp, vp, w)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    step()
+def result(run):
+    for t, s in zip((x, kp, vp, w), state):
+        t.copy_(s)
+    run()
+    K.sync_check()
+    return [t.clone() for t in (x, kp, vp, w, o1, o2, kept, nl, nw, tokens, accepted)]
+a, b = result(g.replay), result(step)
+assert all(torch.equal(m, n) for m, n in zip(a, b))
+print("same")
+"""
+
+
+def test_first_calls_may_be_captured():
+    """Every operator's first call in a process is made while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
 def test_python_refusals(K):
     k, v, table, lens, kv = cache_of(K, [30, 20], 2, 64, 8, F16, 81)
     c = dict(device="cuda")
@@ -607,6 +680,8 @@ def test_python_refusals(K):
     if need:
         with pytest.raises(NrcError):
             K.attn_paged(**ok, workspace=torch.zeros(need - 1, dtype=torch.uint8, **c))
+    with pytest.raises(NrcError):
+        K.attn_paged(**{**ok, "out": torch.zeros(2, 1, 1, 64, **c).expand(2, 1, 4, 64)})
     with pytest.raises(ValueError):
         K.attn_paged(**{**ok, "lens": lens})
     for bad in ((k.cuda(), v.cuda()[:-1], table.cuda()), (k.cuda().float(), v.cuda().float(), table.cuda()),

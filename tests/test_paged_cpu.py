@@ -27,7 +27,8 @@ def desc(**kw):
 BAD_CACHES = [dict(dtype=0), dict(dtype=7), dict(head_dim=48), dict(head_dim=160), dict(head_dim=0), dict(page_size=0),
               dict(n_kv_heads=0), dict(n_seqs=70000), dict(max_pages=2 ** 28, table_stride=2 ** 28), dict(table_stride=1),
               dict(k=FAKE + 8), dict(v=FAKE + 2), dict(page_stride=2052), dict(pos_stride=132), dict(head_stride=68),
-              dict(n_pages=2 ** 31), dict(k=None), dict(table=None), dict(table=FAKE + 2), dict(n_kv_heads=16385)]
+              dict(n_pages=2 ** 31), dict(k=None), dict(table=None), dict(table=FAKE + 2), dict(n_kv_heads=16385),
+              dict(page_stride=0), dict(pos_stride=0), dict(head_stride=0)]
 
 
 def rope(L, kv, dtype=0, tokens=4, heads=4, rot=64, style=1, q=FAKE, freqs=FAKE, pos=FAKE):
