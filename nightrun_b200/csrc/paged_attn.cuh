@@ -142,7 +142,7 @@ NRC_DEV uint32_t units_of(uint32_t len, uint32_t unit = UNIT) { return len ? (le
 // What a (sequence, KV head, row block) costs its first block beside its units: the queries, the first tiles' latency, the
 // join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle (64
 // ragged sequences: 188 us uncounted, 158 us; the tcgen05 kernel on 24: 106 us at 6, 73 us at 14, 76 us at 20).
-constexpr uint32_t SETUP = 2, TC_SETUP = 14;
+constexpr uint32_t SETUP = 2, TC_SETUP = 14, TC_WEIGHTS_SETUP = 6;
 constexpr int TC_TILE = 128;         // rows of a tile of the tcgen05 kernel
 
 // K pieces of a tile: [chunk of 32 values][position g or g + 8].
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
   if (!waited) pdl_wait();
 }
 
-template <bool BF, int HD, int PARTS>
+template <bool BF, int HD, int PARTS, bool WEIGHTS>
 cudaError_t launch_tc(Plan& p, cudaStream_t s);
 
 template <bool BF, int HD, int PARTS, int NT>
@@ -791,7 +791,7 @@ template <bool BF, int HD, int PARTS, int NT>
 cudaError_t launch(Plan& p, cudaStream_t s) {
   void* args[] = {&p};
   cudaError_t err = cudaSuccess;
-  if constexpr (NT == 4 && HD % 64 == 0) err = p.tc ? launch_tc<BF, HD, PARTS>(p, s) : launch_rows<BF, HD, PARTS, NT>(p, s);
+  if constexpr (NT == 4 && HD % 64 == 0) err = p.tc ? launch_tc<BF, HD, PARTS, false>(p, s) : launch_rows<BF, HD, PARTS, NT>(p, s);
   else err = launch_rows<BF, HD, PARTS, NT>(p, s);
   if (err) return err;
   if (!p.direct) {
@@ -802,6 +802,8 @@ cudaError_t launch(Plan& p, cudaStream_t s) {
       return e;
   }
   if (p.a.weights) {
+    if constexpr (NT == 4 && HD % 64 == 0)
+      if (p.tc) return launch_tc<BF, HD, PARTS, true>(p, s);
     return launch_kernel((const void*)k_weights<BF, HD, PARTS, NT>, dim3(p.weight_blocks), dim3(THREADS), 0, s, true, args);
   }
   return cudaSuccess;

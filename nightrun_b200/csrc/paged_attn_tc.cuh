@@ -38,8 +38,8 @@ namespace pattn {
 constexpr int TC_COLS = 32, TC_THREADS = 10 * 32, TC_SOFTMAX = 256;
 constexpr int tc_half(int hd) { return TC_TILE * hd * 2; }  // bytes of a half stage: one tile of K or V
 constexpr int tc_ring(int hd, int parts) { return hd == 64 ? 6 : parts < 3 ? 5 : 4; }
-constexpr int tc_smem(int hd, int parts) {
-  return tc_ring(hd, parts) * tc_half(hd) + 2 * parts * TC_TILE * 64 + parts * TC_COLS * hd * 2 + 1024;
+constexpr int tc_smem(int hd, int parts, bool weights) {
+  return tc_ring(hd, parts) * tc_half(hd) + (weights ? 0 : 2 * parts * TC_TILE * 64) + parts * TC_COLS * hd * 2 + 1024;
 }
 
 NRC_DEV void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
@@ -107,21 +107,28 @@ struct Work {
   uint32_t b, h, rb, len, units, u0, u1, seen;  // seen: positions that every new token sees
   uint32_t tiles;                               // tiles of this piece
 };
-NRC_DEV bool next_work(const Plan& p, Start& st, uint32_t hbs, Work& w) {
+// WEIGHTS: a piece is a KV head's, its row blocks one after the other.
+template <bool WEIGHTS>
+NRC_DEV bool next_work(const Plan& p, Start& st, uint32_t hbs, uint32_t setup, Work& w) {
+  if (WEIGHTS && w.units && w.rb + 1 < p.row_blocks) {
+    w.rb++;
+    return true;
+  }
   if (!st.left) return false;
   w.b = st.b;
-  w.h = st.hb / p.row_blocks;
-  w.rb = st.hb % p.row_blocks;
+  w.h = WEIGHTS ? st.hb : st.hb / p.row_blocks;
+  w.rb = WEIGHTS ? 0 : st.hb % p.row_blocks;
   w.len = seq_len(p, st.b);
   w.units = units_of(w.len, p.tc_tile);
-  const uint32_t v0 = st.unit, v1 = (uint32_t)min((uint64_t)(TC_SETUP + w.units), v0 + st.left);
-  w.u0 = v0 > TC_SETUP ? v0 - TC_SETUP : 0;
-  w.u1 = v1 > TC_SETUP ? v1 - TC_SETUP : 0;
+  const uint32_t v0 = st.unit, v1 = (uint32_t)min((uint64_t)(setup + w.units), v0 + st.left);
+  w.u0 = v0 > setup ? v0 - setup : 0;
+  w.u1 = v1 > setup ? v1 - setup : 0;
   w.seen = w.len > p.a.n_new - 1 ? w.len - (p.a.n_new - 1) : 0;
   const uint32_t end = min(w.u1, (w.seen + p.tc_tile - 1) / p.tc_tile);
   w.tiles = end > w.u0 ? end - w.u0 : 0;
   if (w.u1 == 0) {  // the share ends before the first unit
     st.left = 0;
+    w.units = 0;
     return false;
   }
   st.left -= v1 - v0;
@@ -133,7 +140,9 @@ NRC_DEV bool next_work(const Plan& p, Start& st, uint32_t hbs, Work& w) {
   return true;
 }
 
-template <bool BF, int HD, int PARTS>
+// WEIGHTS: the second pass of calls that add up the positions' weights: the scores again, as exponents above the rows' sums,
+// added over the columns by the thread that owns the position.
+template <bool BF, int HD, int PARTS, bool WEIGHTS>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ Plan p) {
   constexpr int D = tc_ring(HD, PARTS), HALF = tc_half(HD), PB = TC_TILE * 64, NP = TC_COLS * PARTS;
   constexpr uint32_t TMEM = PARTS == 1 ? 128 : PARTS == 2 ? 256 : 512;  // two groups' scores and accumulators
@@ -147,10 +156,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
   __shared__ uint64_t warp_sums[TC_THREADS / 32];
   __shared__ Start start_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t hbs = p.a.kv.n_kv_heads * p.row_blocks;
+  const uint32_t hbs = p.a.kv.n_kv_heads * (WEIGHTS ? 1 : p.row_blocks), setup = WEIGHTS ? TC_WEIGHTS_SETUP : TC_SETUP;
   const uint32_t base = (smem_u32(dyn) + 1023) & ~1023u;
-  const uint32_t ring = base, p_buf = ring + D * HALF, q_buf = p_buf + 2 * PARTS * PB;
-  pdl_trigger();
+  const uint32_t ring = base, p_buf = ring + D * HALF, q_buf = p_buf + (WEIGHTS ? 0 : 2 * PARTS * PB);
+  if (!WEIGHTS) pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < D; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; i++)
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     mbar_init(&drain, 1);
     dead = 0;
     fence_barrier_init();
-    p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (!WEIGHTS) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   for (uint32_t i = threadIdx.x * 16; i < D * HALF; i += TC_THREADS * 16) st_shared16(ring + i, 0, 0, 0, 0);
   fence_proxy_async_smem();  // the rows that no copy fills are zeros
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  Start st = find_start<TC_THREADS>(p, hbs, p.tc_tile, TC_SETUP, warp_sums, &start_s);  // its barriers publish the above
+  Start st = find_start<TC_THREADS>(p, hbs, p.tc_tile, setup, warp_sums, &start_s);  // its barriers publish the above
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   // A wait that runs out ends the kernel's work: whoever sees it tells the others.
@@ -186,7 +195,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     }
     return true;
   };
-  Work w;
+  Work w{};
 
   if (warp == 8) {
     // ---------------------------------------------------------------- copies
@@ -225,7 +234,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       return limit <= r ? 0u : limit - r >= 32 ? 0xffffffffu : (1u << (limit - r)) - 1;
     };
     const uint32_t whole = rows_below(p.tc_tile);
-    while (ok && next_work(p, st, hbs, w)) {
+    while (ok && next_work<WEIGHTS>(p, st, hbs, setup, w)) {
       const uint32_t begin = w.u0 * p.tc_tile, end = min(w.u1 * p.tc_tile, w.seen);
       const int32_t* table = p.a.kv.table + (size_t)w.b * p.a.kv.table_stride;
       // The pages of a batch of tiles, a piece per lane, read one batch ahead.
@@ -276,7 +285,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           __syncwarp();
           copy(&p.k_map, w.h, page, off, there, false, 0);  // K's rows behind the end only make scores that are masked
         }
-        if (i > 0) copy(&p.v_map, w.h, v_page, v_off, v_there, v_cut, v_valid);
+        if (!WEIGHTS && i > 0) copy(&p.v_map, w.h, v_page, v_off, v_there, v_cut, v_valid);
         v_page = page, v_off = off, v_there = there, v_valid = valid, v_cut = cut;
       }
     }
@@ -294,7 +303,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     const Desc q_desc = swizzled_desc(q_buf, 16, 1024, 2), p_desc0 = swizzled_desc(p_buf, PB, 512, 4),
                p_desc1 = swizzled_desc(p_buf + PARTS * PB, PB, 512, 4);
     auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
-    while (ok && next_work(p, st, hbs, w)) {
+    while (ok && next_work<WEIGHTS>(p, st, hbs, setup, w)) {
       if (w.tiles == 0) continue;  // nor do the softmax warps arrive
       ok = all_wait(&q_full, works++ & 1);
       for (uint32_t i = 0; i <= w.tiles && ok; i++) {
@@ -316,7 +325,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           __syncwarp();
           item++;
         }
-        if (i > 0) {
+        if (WEIGHTS && i < w.tiles) {  // no other products
+          if (i & 1)
+            used[1]++;
+          else
+            used[0]++;
+        }
+        if (!WEIGHTS && i > 0) {
           const uint32_t g = (i - 1) & 1, k = g ? used[1] : used[0], slot = item % D;
           ok = all_wait(&full[slot], (item / D) & 1) && all_wait(&p_full[g], k & 1);
           if (!ok) break;
@@ -352,7 +367,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     const uint32_t s_tm = lane_base + g * NP, o_tm = lane_base + 2 * NP;
     uint32_t used = 0, tile = 0;
     bool ok = true, first = true;
-    while (next_work(p, st, hbs, w)) {
+    if (WEIGHTS) pdl_wait();  // the sums below are the kernels' before
+    while (next_work<WEIGHTS>(p, st, hbs, setup, w)) {
       // Queries: 8 threads per row, as in load_queries().
       {
         constexpr int VALUES = HD / 8;
@@ -386,7 +402,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         if (part == 0) {
           const float f = ldexpf(p.a.scale * 1.44269504088896340736f, e);
           fac_s[qr] = f;
-          ref_s[0][qr] = ref_s[1][qr] = UNSET;
+          float ref = UNSET;
+          if (WEIGHTS) {  // a row that is none, or saw nothing, adds nothing
+            const float lse = real ? p.lse[((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.rows + r] : -INFINITY;
+            ref = lse == -INFINITY ? -INFINITY : -lse;
+          }
+          ref_s[0][qr] = ref_s[1][qr] = ref;
         }
         fence_proxy_async_smem();
         if (w.tiles) mbar_arrive(&q_full);
@@ -441,6 +462,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           }
         };
         exponents();
+        if constexpr (WEIGHTS) {
+          tc_fence_before();
+          mbar_arrive(&s_empty[g]);
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int c = 0; c < TC_COLS / 2; c++) sum = __fadd2_rn(sum, make_float2(exp2_fast(x[c].x), exp2_fast(x[c].y)));
+          if (mine) p.a.weights[((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.a.weights_len + (w.u0 + i) * p.tc_tile + row] += sum.x + sum.y;
+          used++;
+          continue;
+        }
         if (sync_any(1 + g, 128, mine && over > LIFT + SLACK)) {
           // New references: each column's largest exponent of the tile, over the lanes, then the warps. Where a row has no
           // reference yet the exponents say nothing: they are taken with reference 0.
@@ -511,10 +542,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         used++;
       }
       tile += w.tiles;
-      if (ok && used != used0) ok = wait(&p_done[g], (used - 1) & 1);
+      if (!WEIGHTS && ok && used != used0) ok = wait(&p_done[g], (used - 1) & 1);
       tc_fence_after();
       // Sums over the positions: lanes, then (below) warps and groups.
-      l_s[g][quarter][lane] = over_lanes(l, lane, [](float a, float b) { return a + b; });
+      if (!WEIGHTS) l_s[g][quarter][lane] = over_lanes(l, lane, [](float a, float b) { return a + b; });
       // The last positions, seen by some of the new tokens only: one (row, position) pair per thread and step.
       if (tail) {
         for (uint32_t i = threadIdx.x; i < TC_COLS * tail; i += TC_SOFTMAX) {
@@ -539,6 +570,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       if (sync_any(3, TC_SOFTMAX, !ok)) {  // sums, tail scores; both groups' products are done
         ok = false;
         break;
+      }
+      if constexpr (WEIGHTS) {
+        if (threadIdx.x < tail) {  // rows in order
+          float sum = 0.0f;
+          for (int c = 0; c < TC_COLS; c++) {
+            const float t = tail_s[c][threadIdx.x];
+            if (t != -INFINITY) sum += exp2_fast(t + ref_s[0][c]);
+          }
+          if (tail_off[threadIdx.x] >= 0)
+            p.a.weights[((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.a.weights_len + w.seen + threadIdx.x] += sum;
+        }
+        named_sync(3, TC_SOFTMAX);
+        continue;
       }
       // Per column: the common reference, the groups' factors, the whole sum; the tail's scores become weights.
       const bool complete = w.u0 == 0 && last, have1 = w.tiles > 1, have0 = w.tiles > 0;
@@ -633,12 +677,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
 }
 
-template <bool BF, int HD, int PARTS>
+template <bool BF, int HD, int PARTS, bool WEIGHTS>
 cudaError_t launch_tc(Plan& p, cudaStream_t s) {
   void* args[] = {&p};
-  const void* fn = (const void*)k_attn_tc<BF, HD, PARTS>;
-  if (cudaError_t e = ensure_smem_attr(fn, tc_smem(HD, PARTS))) return e;
-  return launch_kernel(fn, dim3(p.blocks), dim3(TC_THREADS), tc_smem(HD, PARTS), s, false, args);
+  const void* fn = (const void*)k_attn_tc<BF, HD, PARTS, WEIGHTS>;
+  constexpr int smem = tc_smem(HD, PARTS, WEIGHTS);
+  if (cudaError_t e = ensure_smem_attr(fn, smem)) return e;
+  return launch_kernel(fn, dim3(p.blocks), dim3(TC_THREADS), smem, s, WEIGHTS, args);
 }
 
 }  // namespace pattn
