@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 5 : 2) k_verify_draft
   const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const uint32_t b = blockIdx.x / blocks, m = a.n_max;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
   if (warp == 0) {
     // All drafts at once; the first that is refused counts.
     const int asked = a.n_draft ? a.n_draft[b] : (int)m, nd = asked < 0 ? 0 : asked > (int)m ? (int)m : asked;
@@ -263,6 +264,9 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 5 : 2) k_verify_draft
                          : nullptr;
   row.certain = refused && !a.q ? a.draft[(size_t)b * m + taken] : -1;
   const float u = a.u[(size_t)b * (m + 1) + m];
+
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all have: their shared memory may be written
 
   // Spans of whole 16-byte pieces (counted from the row's start), in index order over blocks and warps.
   const uint32_t spans = blocks * WARPS, per = ((a.vocab + spans - 1) / spans + 7) & ~7u;
