@@ -47,7 +47,8 @@ extern "C" {
 /* Last error message of the calling thread ("" if none). */
 const char* nrc_last_error(void);
 /* Synchronize `stream` and report (then clear) any error a kernel-level entry point's kernel
- * recorded on the current device (NRC_ERR_DEVICE: a bounded wait expired). */
+ * recorded on the current device (NRC_ERR_DEVICE: a bounded wait expired, or a page id, length or
+ * slot lay outside the paged cache). */
 int nrc_sync_check(void* stream);
 /* Diagnostic with no counterpart in the reference: runs one kernel whose bounded wait can never be
  * satisfied (kind 0: an mbarrier arrival withheld; kind 1: a shared-memory flag never raised) and
@@ -209,7 +210,7 @@ int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* args, void* str
  *   out = sum_t p_t V_t,  p = softmax(scale * q . K_t),
  * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into as
  * many cache-typed parts as hold all the bits of `dtype`. q and out: [n_seqs][n_new][n_heads]
- * [head_dim] of `dtype`; lens: int32 [n_seqs]. weights (or NULL): f32 [n_seqs][kv heads][weights_len];
+ * [head_dim] of `dtype`, apart from each other; lens: int32 [n_seqs]. weights (or NULL): f32 [n_seqs][kv heads][weights_len];
  * the weight that a position received from all the query heads of the KV head and all new tokens is
  * added to it. max_len: no sequence is longer (0: the table's width). workspace:
  * nrc_attn_paged_workspace bytes, 16-byte aligned, used by one call at a time. */
@@ -234,7 +235,8 @@ int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* args, void* stre
  * place. kept: int32 [n_seqs][kv heads][budget], the old slots in ascending order, -1 behind a
  * shorter sequence's; new_lens[s] = min(lens[s], budget); new_weights[s][h] = the weights of the kept
  * positions, then zeros. weights and new_weights: f32 [n_seqs][kv heads][weights_len].
- * new_lens == lens and new_weights == weights are allowed. sinks + recent <= budget <= weights_len. */
+ * new_lens == lens and new_weights == weights are allowed. The pages of a sequence longer than budget
+ * belong to it alone. sinks + recent <= budget <= weights_len. */
 int nrc_kv_evict(const nrc_paged_kv* kv, int32_t* kept, int32_t* new_lens, float* new_weights, const int32_t* lens,
                  const float* weights, size_t weights_len, size_t budget, size_t recent, size_t sinks, void* stream);
 /* Drafted tokens against the target, beside nrc_sample: row i of p is the target's distribution

@@ -137,6 +137,7 @@ int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* r, void* stream)
   if (need && (!r->workspace || r->workspace_bytes < need || !aligned16(r->workspace)))
     return nrc_fail_api(NRC_ERR_INVALID, "workspace of %llu bytes, 16-byte aligned: %zu needed",
                         r->workspace ? (unsigned long long)r->workspace_bytes : 0ull, need);
+  if (r->out == r->q) return nrc_fail_api(NRC_ERR_INVALID, "out and q overlap");  // q is read again for the weights
   return cuda_rc(paged_attn_run(a, static_cast<cudaStream_t>(stream)), "attn_paged");
 }
 

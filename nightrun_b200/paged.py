@@ -146,7 +146,7 @@ def attn_paged_workspace(q, kv, weights=False, max_len=0):
 
 def attn_paged(out, q, kv, lens, scale, weights=None, max_len=0, workspace=None, stream=None):
     """Attention (infer.rs:553-572) of the newest tokens of every sequence over its pages: q and out
-    [seqs, new, heads, head_dim] ([seqs, heads, head_dim] for one token each), lens int32 [seqs]
+    [seqs, new, heads, head_dim] ([seqs, heads, head_dim] for one token each; not the same memory), lens int32 [seqs]
     counting the new tokens too; token i of `new` sees the positions before lens - (new - 1 - i), one
     that sees nothing gets zeros. weights (float32 [seqs, KV heads, slots]): what every position
     received is added to it. max_len: no sequence is longer (0: the table's width). Without a
@@ -197,7 +197,7 @@ def attn_paged(out, q, kv, lens, scale, weights=None, max_len=0, workspace=None,
 def evict(kept, new_lens, new_weights, kv, lens, weights, recent, sinks=0, stream=None):
     """Shrinks every sequence longer than kept.shape[2] to that many positions, for each KV head the
     first `sinks`, the latest `recent` and those of largest weight (ties: the earlier one), and
-    compacts its pages in place. kept: int32 [seqs, KV heads, budget], the old slots in ascending
+    compacts its pages, which belong to it alone, in place. kept: int32 [seqs, KV heads, budget], the old slots in ascending
     order, -1 behind a shorter sequence's; new_lens int32 [seqs]; weights, new_weights: float32
     [seqs, KV heads, slots]. new_lens may be lens, new_weights may be weights."""
     i = kv.index

@@ -37,8 +37,8 @@ def rope(L, kv, dtype=0, tokens=4, heads=4, rot=64, style=1, q=FAKE, freqs=FAKE,
     return L.nrc_rope_append(kv, args, None)
 
 
-def attn(L, kv, dtype=0, new=1, heads=4, scale=0.125, weights=None, wlen=0, ws=None, wsb=0, q=FAKE, lens=FAKE):
-    args = paged._ATTN_ARGS.pack(FAKE, 256, 256, 64, q or 0, 256, 256, 64, lens or 0, weights or 0, ws or 0, wsb, wlen, 0,
+def attn(L, kv, dtype=0, new=1, heads=4, scale=0.125, weights=None, wlen=0, ws=None, wsb=0, q=FAKE, lens=FAKE, out=2 * FAKE):
+    args = paged._ATTN_ARGS.pack(out, 256, 256, 64, q or 0, 256, 256, 64, lens or 0, weights or 0, ws or 0, wsb, wlen, 0,
                                  new, heads, dtype, scale)
     return L.nrc_attn_paged(kv, args, None)
 
@@ -84,6 +84,11 @@ def test_attn_paged_refusals(L):
     assert L.nrc_attn_paged_workspace(desc(), 1, 4, 0, 0, None) == -1
     assert L.nrc_attn_paged_workspace(desc(), 1, 5, 0, 0, C.byref(need)) == -1
     assert attn(L, desc(n_seqs=0), ws=FAKE, wsb=1 << 40) == 0
+
+
+def test_attn_paged_refuses_queries_as_its_output(L):
+    assert attn(L, desc(), ws=FAKE, wsb=1 << 40, out=FAKE, q=FAKE) == -1
+    assert b"overlap" in L.nrc_last_error()
 
 
 def test_evict_refusals(L):
