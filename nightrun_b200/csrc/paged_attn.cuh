@@ -78,6 +78,16 @@ NRC_DEV void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The tensor cores cut the low bits of their sums off, always towards zero (over 64000 positions that came to 5e-5 of the
+// output), so sums over many tiles are formed outside of them.
+NRC_DEV void add4(float (&to)[4], const float (&d)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float2 s = __fadd2_rn(make_float2(to[i], to[i + 1]), make_float2(d[i], d[i + 1]));
+    to[i] = s.x;
+    to[i + 1] = s.y;
+  }
+}
 NRC_DEV uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -564,9 +574,12 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
           uint32_t pb[PARTS][2];
           weights_operand<BF, PARTS>(pb, s[n], ref[n], l[n]);
 #pragma unroll
-          for (int i = 0; i < PARTS; i++)
+          for (int j = 0; j < MT; j++) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < MT; j++) mma<BF>(acc[j][n], a[j], pb[i][0], pb[i][1]);
+            for (int i = 0; i < PARTS; i++) mma<BF>(d, a[j], pb[i][0], pb[i][1]);
+            add4(acc[j][n], d);
+          }
         }
       } else {
         // Each token's rows are taken from a product with the values behind it cleared.

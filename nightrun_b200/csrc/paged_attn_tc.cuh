@@ -12,10 +12,11 @@
 // of four softmax warps take turns at the tiles, each with its own scores, weights, references and accumulators (joined at
 // the end), so that one computes while the other's products run.
 //
-// Measured, this kernel against mma.sync: 24 sequences of 1000..9001, 40/8 heads of 64, 5 new tokens, f32 over f16: 73
-// against 99 us; 16 of 4096, 32/8 heads of 128, f16: 8 new tokens 74 against 121 us, 4 new tokens 66 against 74 us (4.1
-// TB/s). A piece of work costs some 14 tiles beside its tiles (queries in, the pipeline filled and drained, the tail, the
-// join), which is what bounds it now where sequences are short; the schedule counts them.
+// Measured, this kernel against mma.sync: 24 sequences of 1000..9001, 40/8 heads of 64, 5 new tokens, f32 over f16: 75
+// against 99 us; 16 of 4096, 32/8 heads of 128, f16: 8 new tokens 76 against 121 us, 4 new tokens 70 against 74 us (3.9
+// TB/s). The weights' pass, 24 sequences as above: 38 against 60 us, part of it under the join. A piece of work costs some 14
+// tiles beside its tiles (queries in, the pipeline filled and drained, the tail, the join), which is what bounds it now where
+// sequences are short; the schedule counts them.
 //
 // Roles (10 warps): 0-7 softmax (two groups), 8 brings K and V rows in by TMA (a page piece of tc_rows rows per copy) into a
 // ring of half stages in the order of their use (K0 K1 V0 K2 V1 ...), 9 issues the products. mbarriers hand the stages on;
@@ -35,6 +36,12 @@
 namespace nrc {
 namespace pattn {
 
+// The tensor cores cut the low bits of their sums off, always towards zero: some 4e-8 of the sum per product. So an
+// accumulator takes this many tiles (8 products each), then it is added to an f32 sum beside it and begun anew: every tile
+// for f32 outputs, 16 for the 16-bit ones, whose own rounding is 2^-12 of the value and more. 5 new tokens, 40/8 heads of 64,
+// f32, 16000 and 64000 positions: 6e-7 and 8e-7 off where one accumulator for all tiles was 8e-6 and 3e-5 off; it costs 3% (24
+// sequences of 1000..9001: 75 against 73 us; sums in registers instead of TMEM: 78 us, they spill).
+constexpr uint32_t tc_drain(bool bf, int parts) { return parts == (bf ? 3 : 2) ? 1 : 16; }
 constexpr int TC_COLS = 32, TC_THREADS = 10 * 32, TC_SOFTMAX = 256;
 constexpr int tc_half(int hd) { return TC_TILE * hd * 2; }  // bytes of a half stage: one tile of K or V
 constexpr int tc_ring(int hd, int parts) { return hd == 64 ? 6 : parts < 3 ? 5 : 4; }
@@ -145,7 +152,7 @@ NRC_DEV bool next_work(const Plan& p, Start& st, uint32_t hbs, uint32_t setup, W
 template <bool BF, int HD, int PARTS, bool WEIGHTS>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ Plan p) {
   constexpr int D = tc_ring(HD, PARTS), HALF = tc_half(HD), PB = TC_TILE * 64, NP = TC_COLS * PARTS;
-  constexpr uint32_t TMEM = PARTS == 1 ? 128 : PARTS == 2 ? 256 : 512;  // two groups' scores and accumulators
+  constexpr uint32_t DRAIN = tc_drain(BF, PARTS), TMEM = WEIGHTS ? NP * 2 > 128 ? 256 : 128 : PARTS == 1 ? 256 : 512;  // two groups' scores, accumulators and sums
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[D], empty[D], s_full[2], s_empty[2], p_full[2], p_done[2], q_full, cut_full, drain;
   __shared__ uint32_t tmem_s, dead;
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           tc_fence_after();
           const Desc a = swizzled_desc(ring + slot * HALF, HD == 64 ? 0 : TC_TILE * 128, 1024, 2);
           const Desc b = g ? p_desc1 : p_desc0;
-          const uint32_t d = tmem + (2 + g) * NP, onto = i > 2 ? 1u : 0u;
+          const uint32_t d = tmem + (2 + g) * NP, onto = (i - 1) / 2 % DRAIN;
           if (leader) {
 #pragma unroll
             for (int s = 0; s < TC_TILE / 16; s++) tc_mma_f16(d, a.at(s * 2048), b.at(s * 1024), id_o, s ? 1u : onto);
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     // ---------------------------------------------------------------- softmax
     const int g = warp >> 2, quarter = warp & 3, row = threadIdx.x & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_tm = lane_base + g * NP, o_tm = lane_base + 2 * NP;
+    const uint32_t s_tm = lane_base + g * NP, o_tm = lane_base + 2 * NP, sum_tm = lane_base + 4 * NP + g * TC_COLS;
     uint32_t used = 0, tile = 0;
     bool ok = true, first = true;
     if (WEIGHTS) pdl_wait();  // the sums below are the kernels' before
@@ -424,6 +431,43 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
 #pragma unroll
       for (int c = 0; c < TC_COLS / 2; c++) l[c] = make_float2(0.0f, 0.0f);
       const uint32_t used0 = used;
+      // The accumulator's parts, added to what was drained before; its products are done.
+      auto drained = [&](uint32_t to) {
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint32_t sum[16], o[16];
+          tc_ld16(sum_tm + 16 * h, sum);
+          tc_wait_ld_regs<16>(sum);
+#pragma unroll
+          for (int c = 0; c < 16; c++) sum[c] = used - used0 > DRAIN ? sum[c] : 0u;  // the first time nothing stands there
+#pragma unroll
+          for (int j = 0; j < PARTS; j++) {
+            tc_ld16(o_tm + g * NP + j * TC_COLS + 16 * h, o);
+            tc_wait_ld_regs<16>(o);
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const float2 x = __fadd2_rn(make_float2(__uint_as_float(sum[c]), __uint_as_float(sum[c + 1])),
+                                          make_float2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])));
+              sum[c] = __float_as_uint(x.x);
+              sum[c + 1] = __float_as_uint(x.y);
+            }
+          }
+          tc_st16(to + 16 * h, sum);
+        }
+        tc_wait_st();
+      };
+      auto scaled = [&](uint32_t at) {  // 16 columns by their rows' factors
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint32_t o[16];
+          tc_ld16(at + 16 * h, o);
+          tc_wait_ld_regs<16>(o);
+#pragma unroll
+          for (int c = 0; c < 16; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * f_s[g][16 * h + c]);
+          tc_st16(at + 16 * h, o);
+        }
+      };
       for (uint32_t i = g; i < w.tiles; i += 2) {
         if (ok) ok = wait(&s_full[g], used & 1);
         if (sync_any(1 + g, 128, !ok)) {
@@ -504,14 +548,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             tc_fence_after();
             if (ok) {
 #pragma unroll
-              for (int h = 0; h < 2 * PARTS; h++) {
-                uint32_t o[16];
-                tc_ld16(o_tm + g * NP + 16 * h, o);
-                tc_wait_ld_regs<16>(o);
-#pragma unroll
-                for (int c = 0; c < 16; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * f_s[g][(16 * h + c) % TC_COLS]);
-                tc_st16(o_tm + g * NP + 16 * h, o);
-              }
+              for (int j = 0; j < PARTS; j++) scaled(o_tm + g * NP + j * TC_COLS);
+              if (used - used0 > DRAIN) scaled(sum_tm);
               tc_wait_st();
             }
           }
@@ -522,7 +560,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
 #pragma unroll
           for (int c = 0; c < TC_COLS / 2; c++) x[c] = make_float2(-INFINITY, -INFINITY);
         }
-        if (ok && used) ok = wait(&p_done[g], (used - 1) & 1);  // the weights before are used up
+        if (used) ok = __all_sync(0xffffffffu, ok && wait(&p_done[g], (used - 1) & 1));  // the weights before are used up
+        if (ok && used != used0 && (used - used0) % DRAIN == 0) drained(sum_tm);
         const uint32_t p_row = p_buf + g * PARTS * PB + row * 64;
 #pragma unroll
         for (int c0 = 0; c0 < TC_COLS / 2; c0 += 4) {
@@ -538,12 +577,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             st_shared16(p_row + j * PB + (((c0 / 4) ^ ((row >> 1) & 3)) << 4), v[0][j], v[1][j], v[2][j], v[3][j]);
         }
         fence_proxy_async_smem();
+        tc_fence_before();
         mbar_arrive(&p_full[g]);
         used++;
       }
       tile += w.tiles;
-      if (!WEIGHTS && ok && used != used0) ok = wait(&p_done[g], (used - 1) & 1);
-      tc_fence_after();
+      if (!WEIGHTS && used != used0) {  // the whole sums to the accumulator's first columns, where both groups read them
+        ok = __all_sync(0xffffffffu, ok && wait(&p_done[g], (used - 1) & 1));
+        if (ok) drained(o_tm + g * NP);
+      }
+      tc_fence_before();
       // Sums over the positions: lanes, then (below) warps and groups.
       if (!WEIGHTS) l_s[g][quarter][lane] = over_lanes(l, lane, [](float a, float b) { return a + b; });
       // The last positions, seen by some of the new tokens only: one (row, position) pair per thread and step.
@@ -618,16 +661,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
 #pragma unroll
       for (int k = 0; k < 16; k++) o[k] = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {  // the groups' accumulators and their parts
+      for (int h = 0; h < 2; h++) {  // the groups' sums
         if (h ? !have1 : !have0) continue;
+        uint32_t v[16];
+        tc_ld16(o_tm + h * NP + 16 * g, v);
+        tc_wait_ld_regs<16>(v);
 #pragma unroll
-        for (int j = 0; j < PARTS; j++) {
-          uint32_t v[16];
-          tc_ld16(o_tm + h * NP + j * TC_COLS + 16 * g, v);
-          tc_wait_ld_regs<16>(v);
-#pragma unroll
-          for (int k = 0; k < 16; k++) o[k] = fmaf(f_s[h][16 * g + k], __uint_as_float(v[k]), o[k]);
-        }
+        for (int k = 0; k < 16; k++) o[k] = fmaf(f_s[h][16 * g + k], __uint_as_float(v[k]), o[k]);
       }
       tc_fence_before();
       if (row < HD) {

@@ -279,6 +279,28 @@ def test_attn_paged_many_rows_with_infinities(K):
     assert torch.allclose(out[0, 3, 0].double().cpu(), p @ vv[:, 0], atol=1e-5)
 
 
+@pytest.mark.parametrize("new,d,ct", [(1, 64, F16), (5, 64, F16), (3, 96, F16), (2, 128, BF16)])
+def test_attn_paged_long_sums_lean_to_no_side(K, new, d, ct):
+    """Products on the tensor cores are cut towards zero, so sums of many of them would lean that way. Positive values,
+    scores well below 1: the errors' mean has to stay below what 8 products cut, each up to 2^-23 of a sum that grows to
+    the whole (4.5 of 2^-23 together, under 2^-20); roundings to nearest have no mean."""
+    g = torch.Generator(device="cuda").manual_seed(new)
+    n, page, hq, hk, seqs = 16000, 64, 40, 8, 32
+    k_pages, v_pages = (torch.randn(n // page, page, hk, d, generator=g, device="cuda").to(ct) for _ in range(2))
+    v_pages = v_pages.abs()
+    table = torch.randperm(n // page, generator=g, device="cuda").int().repeat(seqs, 1)  # all read the same pages
+    q = (torch.randn(1, new, hq, d, generator=g, device="cuda") * 0.2).repeat(seqs, 1, 1, 1)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    K.attn_paged(out, q, K.PagedKV(k_pages, v_pages, table), lens, d ** -0.5)
+    keys, values = (x[table[0].long()].reshape(n, hk, d).double() for x in (k_pages, v_pages))
+    s = torch.einsum("nhgd,lhd->hgnl", q[0].double().view(new, hk, hq // hk, d), keys) * d ** -0.5
+    seen = torch.arange(n, device="cuda") < n - (new - 1) + torch.arange(new, device="cuda")[:, None]
+    p = s.masked_fill(~seen, -float("inf")).softmax(-1)
+    want = torch.einsum("hgnl,lhd->nhgd", p, values).reshape(1, new, hq, d)
+    assert float(((out.double() - want).mean((1, 2, 3)) / want.mean()).abs().max()) < 2 ** -20
+
+
 def test_attn_paged_strides_and_shapes(K):
     """q and out inside wider tensors, one token without its dimension, pages laid out by head, a narrow slice of a table."""
     g = gen(13)
