@@ -751,7 +751,9 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
           lse[n][i] = x == -INFINITY ? INFINITY : x;
         }
       for (uint32_t p0 = (u0 * WARPS + warp) * TILE; p0 < end; p0 += UNIT) {
-        float s[NT][4], sum[2] = {0.0f, 0.0f};
+        float s[NT][4], sum[2] = {0.0f, 0.0f}, before[2];  // before: what stands at its positions
+#pragma unroll
+        for (int i = 0; i < 2; i++) before[i] = t == 0 && p0 + g + 8 * i < end ? w[p0 + g + 8 * i] : 0.0f;
         scores<BF, HD, PARTS, NT>(s, k, qs, lane);
         walk.next(p);
         walk.load_k<HD>(k, lane);
@@ -774,7 +776,7 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
           const uint32_t r = g + 8 * i;
-          if (t == 0 && p0 + r < end && ((ok >> r) & 1)) w[p0 + r] += sum[i];
+          if (t == 0 && p0 + r < end && ((ok >> r) & 1)) w[p0 + r] = before[i] + sum[i];
         }
       }
     }

@@ -14,7 +14,7 @@
 //
 // Measured, this kernel against mma.sync: 24 sequences of 1000..9001, 40/8 heads of 64, 5 new tokens, f32 over f16: 75
 // against 99 us; 16 of 4096, 32/8 heads of 128, f16: 8 new tokens 76 against 121 us, 4 new tokens 70 against 74 us (3.9
-// TB/s). The weights' pass, 24 sequences as above: 38 against 60 us, part of it under the join. A piece of work costs some 14
+// TB/s). The weights' pass, 24 sequences as above: 35 against 60 us, part of it under the join. A piece of work costs some 14
 // tiles beside its tiles (queries in, the pipeline filled and drained, the tail, the join), which is what bounds it now where
 // sequences are short; the schedule counts them.
 //
@@ -469,6 +469,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         }
       };
       for (uint32_t i = g; i < w.tiles; i += 2) {
+        float before = 0.0f;  // what stands at this thread's position: on its way while the scores are formed
+        float* weight = nullptr;
+        if constexpr (WEIGHTS) {
+          const uint32_t pos = (w.u0 + i) * p.tc_tile + row;
+          weight = p.a.weights + ((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.a.weights_len + pos;
+          if ((uint32_t)row < p.tc_tile && pos < w.seen) before = *weight;
+        }
         if (ok) ok = wait(&s_full[g], used & 1);
         if (sync_any(1 + g, 128, !ok)) {
           ok = false;
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int c = 0; c < TC_COLS / 2; c++) sum = __fadd2_rn(sum, make_float2(exp2_fast(x[c].x), exp2_fast(x[c].y)));
-          if (mine) p.a.weights[((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.a.weights_len + (w.u0 + i) * p.tc_tile + row] += sum.x + sum.y;
+          if (mine) *weight = before + (sum.x + sum.y);
           used++;
           continue;
         }
