@@ -151,7 +151,8 @@ NRC_DEV uint32_t seq_len(const Plan& p, uint32_t b) {
 NRC_DEV uint32_t units_of(uint32_t len, uint32_t unit = UNIT) { return len ? (len + unit - 1) / unit : 1u; }
 // What a (sequence, KV head, row block) costs its first block beside its units: the queries, the first tiles' latency, the
 // join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle (64
-// ragged sequences: 188 us uncounted, 158 us; the tcgen05 kernel on 24: 106 us at 6, 73 us at 14, 76 us at 20).
+// ragged sequences: 188 us uncounted, 158 us; the tcgen05 kernel on 24: 106 us at 6, 73 us at 14, 76 us at 20; its weights'
+// pass 39 us at 3, 35 us at 6, 37 us at 12).
 constexpr uint32_t SETUP = 2, TC_SETUP = 14, TC_WEIGHTS_SETUP = 6;
 constexpr int TC_TILE = 128;         // rows of a tile of the tcgen05 kernel
 
