@@ -42,6 +42,10 @@ namespace pattn {
 // f32, 16000 and 64000 positions: 6e-7 and 8e-7 off where one accumulator for all tiles was 8e-6 and 3e-5 off; it costs 3% (24
 // sequences of 1000..9001: 75 against 73 us; sums in registers instead of TMEM: 78 us, they spill).
 constexpr uint32_t tc_drain(bool bf, int parts) { return parts == (bf ? 3 : 2) ? 1 : 16; }
+// Tiles whose masks are kept. The copying warp writes tile T's before it waits for T's ring slot: it knows then that the
+// products of tile T - 1 - D are done (in the weights' pass, where only K goes through the ring of D), hence that the scores
+// two tiles before that have been read, and the masks with them. T - 2 - D may still be waiting to be: D + 3 at least.
+constexpr int TC_MASKS = 16;
 constexpr int TC_COLS = 32, TC_THREADS = 10 * 32, TC_SOFTMAX = 256;
 constexpr int tc_half(int hd) { return TC_TILE * hd * 2; }  // bytes of a half stage: one tile of K or V
 constexpr int tc_ring(int hd, int parts) { return hd == 64 ? 6 : parts < 3 ? 5 : 4; }
@@ -156,7 +160,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[D], empty[D], s_full[2], s_empty[2], p_full[2], p_done[2], q_full, cut_full, drain;
   __shared__ uint32_t tmem_s, dead;
-  __shared__ uint32_t cached_s[8][4];                 // which positions of a tile are cached, by tile number
+  static_assert(TC_MASKS >= D + 3, "the copies would overwrite the mask of a tile that is still to be read");
+  __shared__ uint32_t cached_s[TC_MASKS][4];          // which positions of a tile are cached, by tile number
   __shared__ __align__(16) float fac_s[TC_COLS], ref_s[2][TC_COLS];  // factor of each row, its reference per group
   __shared__ float f_s[2][TC_COLS], old_s[2][TC_COLS], top_s[2][4][TC_COLS], l_s[2][4][TC_COLS], tail_s[TC_COLS][17], sum_s[TC_COLS];
   __shared__ int64_t tail_off[16];
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
                 if (lane == q) valid = word;
               }
           }
-          if (lane < 4) cached_s[tile % 8][lane] = valid;
+          if (lane < 4) cached_s[tile % TC_MASKS][lane] = valid;
           tile++;
           if (++j == batch) j = 0;
           __syncwarp();
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         }
         __syncwarp();
         tc_fence_after();
-        const uint32_t there = cached_s[(tile + i) % 8][quarter];
+        const uint32_t there = cached_s[(tile + i) % TC_MASKS][quarter];
         const bool mine = (there >> lane) & 1;
         float2 x[TC_COLS / 2];  // exponents of neighbouring columns
         float over = -INFINITY;
