@@ -353,17 +353,14 @@ int nrc_sync_check(void* stream) {
   unsigned paged = 0, attn = 0;
   if (paged_take_errors(&paged) != cudaSuccess || paged_attn_take_errors(&attn) != cudaSuccess)
     return nrc_fail_api(NRC_ERR_CUDA, "read error word");
-  if (err) {
-    cudaMemset(sc.err, 0, 4);
-    return nrc_fail_api(NRC_ERR_DEVICE, "kernel wait expired (error bits 0x%x)", err);
-  }
-  if (paged | attn)
-    return nrc_fail_api(NRC_ERR_DEVICE, "%s (error bits 0x%x)",
-                        (paged | attn) & ERR_BAD_PAGE   ? "a page id outside the pool"
-                        : (paged | attn) & ERR_BAD_SLOT ? "a length, sequence or slot outside the table"
-                                                        : "kernel wait expired",
-                        paged | attn);
-  return NRC_OK;
+  if (err) cudaMemset(sc.err, 0, 4);
+  const unsigned all = err | paged | attn;  // all three words are cleared: one message names what they held
+  if (!all) return NRC_OK;
+  const bool page = (paged | attn) & ERR_BAD_PAGE, slot = (paged | attn) & ERR_BAD_SLOT;
+  const bool wait = err || ((paged | attn) & ~(ERR_BAD_PAGE | ERR_BAD_SLOT));
+  return nrc_fail_api(NRC_ERR_DEVICE, "%s%s%s%s%s (error bits 0x%x)", wait ? "kernel wait expired" : "",
+                      wait && (page || slot) ? "; " : "", page ? "a page id outside the pool" : "", page && slot ? "; " : "",
+                      slot ? "a length, sequence or slot outside the table" : "", all);
 }
 
 }  // extern "C"

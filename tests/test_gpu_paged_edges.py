@@ -75,3 +75,21 @@ def test_weights_of_long_pieces(K, seqs, shortest, longest, new, hq, hk, d, dt, 
         whole = w0[s, :, :m].double() + want
         assert bool(((first[0][s, :, :m].double() - whole).abs() <= want * rel + whole * 2.0 ** -23).all())
         assert torch.equal(first[0][s, :, m:], w0[s, :, m:])
+
+
+# ------------------------------------------------------------------ errors
+
+
+def test_errors_of_several_kernels_are_all_reported(K):
+    """A page outside the pool and a slot outside the table, then a wait that runs out: one report names all three."""
+    from nightrun_b200._lib import lib
+    k, v, table = R.make_pages(gen(1), 2, 2, 4, 1, 32, F16)
+    table[0, 1] = 10 ** 6
+    kv = K.PagedKV(k.cuda(), v.cuda(), table.cuda())
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    x, freqs = torch.zeros(2, 1, 32, device="cuda"), torch.tensor(K.rope_freqs(32, 10000.0), device="cuda")
+    K.rope_append(x, x, x.clone(), x.clone(), kv, freqs, i32(0, 1), i32(0, 1), i32(4, 8))
+    assert lib().nrc_wait_selftest(0, 20_000_000, None) == -4
+    message = lib().nrc_last_error().decode()
+    assert "wait expired" in message and "page id" in message and "slot" in message
+    K.sync_check()  # reported once
