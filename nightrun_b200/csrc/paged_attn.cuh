@@ -350,6 +350,43 @@ NRC_DEV void load_queries(const Plan& p, uint32_t b, uint32_t h, uint32_t rb, Qu
   if (part == 0) qs.factor[row] = ldexpf(p.a.scale * 1.44269504088896340736f, e);
 }
 
+// q . K_t in f32, value after value, of the query row that begins at element `at` and a cached row: the definition's way, for
+// what the tensor cores' operands cannot hold. q as it was given.
+template <bool BF, int HD>
+NRC_DEV float dot_row(const Plan& p, int64_t at, const uint4* k) {
+  float d = 0.0f;
+#pragma unroll 4
+  for (int c = 0; c < HD / 8; c++) {
+    const uint4 w = k[c];
+#pragma unroll
+    for (int e = 0; e < 8; e++) d = fmaf(load_as_f32(p.a.q, at + 8 * c + e, p.a.dtype), load_as_f32(&w, e, BF ? NRC_BF16 : NRC_F16), d);
+  }
+  return d;
+}
+NRC_DEV int64_t query_row(const Plan& p, uint32_t b, uint32_t h, uint32_t r) {
+  return (int64_t)b * p.a.q_seq + (int64_t)(r / p.gqa) * p.a.q_token + (int64_t)(h * p.gqa + r % p.gqa) * p.a.q_head;
+}
+NRC_DEV const uint4* cached_row(const void* rows, int64_t row, const Plan& p, uint32_t h) {
+  return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(rows) + row + (int64_t)h * p.a.kv.head_stride);
+}
+
+// What position t receives from the query rows [r0, r1), formed anew in f32 where the tensor cores' sum is no number: an
+// infinite key times the zeros of a column that is no row is NaN there, and so is an infinite key times the parts of a split
+// query. A row that is NaN itself leaves NaN.
+template <bool BF, int HD>
+__device__ __noinline__ float weight_again(const Plan& p, uint32_t b, uint32_t h, uint32_t r0, uint32_t r1, uint32_t len, uint32_t t) {
+  const float* lse = p.lse + ((size_t)b * p.a.kv.n_kv_heads + h) * p.rows;
+  const int64_t row = paged_row(p.a.kv, b, t);
+  float sum = 0.0f;
+  for (uint32_t r = r0; r < r1 && sum == sum; r++) {
+    const float l = lse[r];
+    if (t + (p.a.n_new - 1 - r / p.gqa) >= len || l == -INFINITY) continue;
+    const float d = l == l ? dot_row<BF, HD>(p, query_row(p, b, h, r), cached_row(p.a.kv.k, row, p, h)) : l;
+    sum += exp2_fast(fmaf(d, p.a.scale * 1.44269504088896340736f, -l));
+  }
+  return sum;
+}
+
 // S^T of a tile. Few columns: two chains of products, so that one's latency hides the other's.
 template <bool BF, int HD, int PARTS, int NT>
 NRC_DEV void scores(float (&s)[NT][4], const KTile<HD>& k, const Queries<HD, PARTS, NT>& qs, int lane) {
@@ -777,7 +814,10 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __g
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
           const uint32_t r = g + 8 * i;
-          if (t == 0 && p0 + r < end && ((ok >> r) & 1)) w[p0 + r] = before[i] + sum[i];
+          if (t == 0 && p0 + r < end && ((ok >> r) & 1)) {
+            if (!(sum[i] < INFINITY)) sum[i] = weight_again<BF, HD>(p, b, h, rb * COLS, min(p.rows, (rb + 1) * COLS), len, p0 + r);
+            w[p0 + r] = before[i] + sum[i];
+          }
         }
       }
     }

@@ -524,7 +524,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int c = 0; c < TC_COLS / 2; c++) sum = __fadd2_rn(sum, make_float2(exp2_fast(x[c].x), exp2_fast(x[c].y)));
-          if (mine) *weight = before + (sum.x + sum.y);
+          float add = sum.x + sum.y;
+          if (mine && !(add < INFINITY))
+            add = weight_again<BF, HD>(p, w.b, w.h, w.rb * TC_COLS, min(p.rows, (w.rb + 1) * TC_COLS), w.len, (w.u0 + i) * p.tc_tile + row);
+          if (mine) *weight = before + add;
           used++;
           continue;
         }
@@ -607,17 +610,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           const uint32_t c = i / tail, j = i - c * tail, r = w.rb * TC_COLS + c, tok = r / p.gqa;
           float x = -INFINITY;
           if (r < p.rows && w.seen + j + (p.a.n_new - 1 - tok) < w.len && tail_off[j] >= 0) {
-            const int64_t at = (int64_t)w.b * p.a.q_seq + (int64_t)tok * p.a.q_token + (int64_t)(w.h * p.gqa + r % p.gqa) * p.a.q_head;
             const uint4* kr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a.kv.k) + tail_off[j]);
-            float d = 0.0f;
-#pragma unroll 4
-            for (int k = 0; k < HD / 8; k++) {
-              const uint4 kw = kr[k];
-#pragma unroll
-              for (int e = 0; e < 8; e++)
-                d = fmaf(load_as_f32(p.a.q, at + 8 * k + e, p.a.dtype), load_as_f32(&kw, e, BF ? NRC_BF16 : NRC_F16), d);
-            }
-            x = d * (p.a.scale * 1.44269504088896340736f);
+            x = dot_row<BF, HD>(p, query_row(p, w.b, w.h, r), kr) * (p.a.scale * 1.44269504088896340736f);
           }
           tail_s[c][j] = x;
         }

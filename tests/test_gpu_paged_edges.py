@@ -93,3 +93,96 @@ def test_errors_of_several_kernels_are_all_reported(K):
     message = lib().nrc_last_error().decode()
     assert "wait expired" in message and "page id" in message and "slot" in message
     K.sync_check()  # reported once
+
+
+# ------------------------------------------------------------------ infinities and NaN in the cache
+
+
+def expected(q, k_pages, v_pages, table, lens, scale):
+    """out, weights and their tolerances, in 64 bits and by IEEE's rules: a score of -inf has weight 0, one of +inf or NaN
+    leaves NaN in its row, an infinite value at a position of weight above 0 is the output's.
+
+    Scores: d products, summed in f32 one after the other at worst, (d + 8) 2^-24 of the sum of magnitudes, and operands
+    that hold 2^-22 of theirs; weights and sums as in R.attention_tolerance."""
+    b, n, hq, d = q.shape
+    hk, slots = k_pages.shape[2], table.shape[1] * k_pages.shape[1]
+    g = hq // hk
+    out, tol = torch.zeros(b, n, hq, d, dtype=torch.float64), torch.zeros(b, n, hq, d, dtype=torch.float64)
+    weights, wtol = torch.zeros(b, hk, slots, dtype=torch.float64), torch.zeros(b, hk, slots, dtype=torch.float64)
+    enter = 2.0 ** -22 if q.dtype == F32 else 2.0 ** -16 if R.HALF[q.dtype] < R.HALF[k_pages.dtype] else R.HALF[k_pages.dtype]
+    for s in range(b):
+        m = int(lens[s])
+        keys, values = (R.rows(x, table, s, range(m)).double() for x in (k_pages, v_pages))
+        for j in range(n):
+            sees = m - (n - 1 - j)
+            if sees <= 0:
+                continue
+            for h in range(hq):
+                kk, vv, qq = keys[:sees, h // g], values[:sees, h // g], q[s, j, h].double()
+                x = (kk * qq).sum(1) * scale
+                p = torch.softmax(x, 0)
+                out[s, j, h] = (p[:, None] * vv).sum(0)
+                big = ((kk * qq).abs().sum(1) * abs(scale)).nan_to_num(0.0, 0.0, 0.0).max()
+                delta = big * ((d + 8) * 2.0 ** -24 + 2.0 ** -22)
+                sums = (3 * sees / 16 + 40) * 2.0 ** -23
+                size = (p[:, None] * vv.abs()).nan_to_num(0.0, 0.0, 0.0).sum(0)
+                tol[s, j, h] = (size * (2.2 * delta + enter + 2.0 ** -20 + 2 * sums)
+                                + out[s, j, h].abs().nan_to_num(0.0, 0.0, 0.0) * R.HALF[q.dtype] + R.TINY[q.dtype])
+                weights[s, h // g, :sees] += p
+                wtol[s, h // g, :sees] += p * (2.2 * delta + 2.0 ** -20 + sums + 2.0 ** -21)
+    return out, tol, weights, wtol
+
+
+def same(got, want, tol):
+    """Finite where `want` is and within `tol` there, the same infinities, NaN where NaN."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    at = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), at) and torch.equal(got[at], want[at])
+    fine = torch.isfinite(want)
+    assert bool(((got - want).abs()[fine] <= tol[fine]).all())
+
+
+ODD = [  # lens, new, heads, kv heads, dim, type, cache, page
+    ([70, 48], 1, 8, 2, 64, F16, F16, 16), ([70, 48], 1, 8, 2, 64, F32, F16, 16),         # unsplit; 4 of 8 columns
+    ([700, 301], 1, 10, 2, 128, BF16, BF16, 16), ([700, 301], 1, 8, 2, 128, F32, BF16, 7),  # split and joined
+    ([400], 3, 8, 2, 96, F16, BF16, 24), ([333, 90], 3, 6, 2, 32, F32, F16, 9),             # 12 and 9 rows off tcgen05
+    ([700, 513], 3, 8, 2, 64, F32, F16, 16), ([640, 300], 4, 6, 2, 64, F16, F16, 24),       # tcgen05
+    ([700, 400], 3, 8, 2, 128, F16, BF16, 64), ([650], 4, 20, 2, 128, BF16, BF16, 32)]
+
+
+def odd_case(K, case, seed):
+    lens, new, hq, hk, d, dt, ct, page = case
+    g = gen(seed)
+    k, v, table = R.make_pages(g, len(lens), -(-max(lens) // page) + 1, page, hk, d, ct)
+    q = torch.randn(len(lens), new, hq, d, generator=g).to(dt)
+    return q, k, v, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def run_odd(K, q, k, v, table, lens, scale):
+    kv = K.PagedKV(k.cuda(), v.cuda(), table.cuda())
+    w = torch.zeros(len(lens), k.shape[2], table.shape[1] * k.shape[1], device="cuda")
+    out = torch.empty_like(q, device="cuda")
+    K.attn_paged(out, q.cuda(), kv, lens.cuda(), scale, weights=w)
+    alone = torch.empty_like(out)
+    K.attn_paged(alone, q.cuda(), kv, lens.cuda(), scale)
+    assert torch.equal(alone.isnan(), out.isnan()) and torch.equal(alone.nan_to_num(7.0), out.nan_to_num(7.0))
+    return out, w
+
+
+@pytest.mark.parametrize("case", [c for c in ODD if c[5] == c[6]], ids=lambda c: str(ODD.index(c)))
+def test_infinite_keys_that_count_for_nothing(K, case):
+    """Keys that are infinite where every query is below zero: their scores are -inf, their weights 0, and nothing else
+    changes, whatever columns of a tile are no rows."""
+    q, k, v, table, lens = odd_case(K, case, 31)
+    q[..., 5] = -q[..., 5].abs().clamp(min=0.01)
+    for s, n in enumerate(lens.tolist()):
+        for t in (0, 17, n // 2, n - 1):
+            row = R.rows(k, table, s, [t])[0].clone()
+            row[:, 5] = INF
+            R.put(k, table, s, t, row)
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.2)
+    assert torch.isfinite(want).all() and torch.isfinite(ww).all()
+    out, w = run_odd(K, q, k, v, table, lens, 0.2)
+    same(w, ww, wtol + 1e-30)
+    same(out, want, tol)
