@@ -350,6 +350,11 @@ NRC_DEV void load_queries(const Plan& p, uint32_t b, uint32_t h, uint32_t rb, Qu
   if (part == 0) qs.factor[row] = ldexpf(p.a.scale * 1.44269504088896340736f, e);
 }
 
+// A score's exponential is taken as 2^(s + ref): ref is LIFT less the largest score seen when the row's reference was last
+// set, and is set again (its sums rescaled) when an exponent passes LIFT + SLACK, so most tiles need no reduction over
+// their positions. f16 weights: up to 2^15, and with bits down to 2^-24, 2^-32 of the row's sum. UNSET: nothing seen.
+constexpr float SLACK = 7.0f, LIFT = 8.0f, UNSET = 3e38f;
+
 // q . K_t in f32, value after value, of the query row that begins at element `at` and a cached row: the definition's way, for
 // what the tensor cores' operands cannot hold. q as it was given.
 template <bool BF, int HD>
@@ -385,6 +390,70 @@ __device__ __noinline__ float weight_again(const Plan& p, uint32_t b, uint32_t h
     sum += exp2_fast(fmaf(d, p.a.scale * 1.44269504088896340736f, -l));
   }
   return sum;
+}
+
+// A row of a piece of work, the positions [begin, end), formed anew in f32 by one warp where the tensor cores' sums are no
+// numbers: there an infinite key or value meets the parts of a split operand (inf - inf), a weight that 16 bits round to 0,
+// or the weight 0 of a row that does not see it. Here it counts by IEEE's rules: a score of -inf has weight 0, an infinite
+// value of weight above 0 is the output's, a position that the row does not see is left out. Written where the piece's
+// results go: to part_row of the partial results, or (part_row < 0) to the output. A lane takes a position for the scores, HD / 32
+// values for the sums.
+template <bool BF, int HD>
+__device__ __noinline__ void row_again(const Plan& p, uint32_t b, uint32_t h, uint32_t r, uint32_t begin, uint32_t end,
+                                       int64_t part_row) {
+  constexpr int VALUES = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t len = seq_len(p, b), behind = p.a.n_new - 1 - r / p.gqa;
+  end = min(end, len > behind ? len - behind : 0);
+  auto score = [&](uint32_t t, int64_t& row) {
+    row = t < end ? paged_row(p.a.kv, b, t) : -1;
+    if (row < 0) return -INFINITY;
+    return dot_row<BF, HD>(p, query_row(p, b, h, r), cached_row(p.a.kv.k, row, p, h)) * (p.a.scale * 1.44269504088896340736f);
+  };
+  float top = -INFINITY, sum = 0.0f, o[VALUES] = {};
+  int64_t row;
+  bool none = false;  // no number: a score of NaN or +inf
+  for (uint32_t t0 = begin; t0 < end && !none; t0 += 32) {
+    const float s = score(t0 + lane, row);
+    top = fmaxf(top, s);
+    none = __any_sync(0xffffffffu, !(s < INFINITY));
+  }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+  const float low = none || top == -INFINITY ? UNSET : -top;
+  for (uint32_t t0 = begin; t0 < end && !none; t0 += 32) {
+    const float s = score(t0 + lane, row), e = exp2_fast(s + low);
+    sum += e;
+    float part[VALUES] = {};
+    for (uint32_t j = 0; j < min(32u, end - t0); j++) {
+      const int64_t at = __shfl_sync(0xffffffffu, row, j);
+      const float weight = __shfl_sync(0xffffffffu, e, j);
+      if (at < 0) continue;
+#pragma unroll
+      for (int i = 0; i < VALUES; i++)
+        part[i] = fmaf(weight, load_as_f32(cached_row(p.a.kv.v, at, p, h), lane + 32 * i, BF ? NRC_BF16 : NRC_F16), part[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VALUES; i++) o[i] += part[i];
+  }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+  if (none) sum = __int_as_float(0x7fffffff);
+#pragma unroll
+  for (int i = 0; i < VALUES; i++) {
+    if (none) o[i] = sum;
+    if (part_row < 0)
+      store_from_f32(p.a.out,
+                     (int64_t)b * p.a.o_seq + (int64_t)(r / p.gqa) * p.a.o_token + (int64_t)(h * p.gqa + r % p.gqa) * p.a.o_head + lane + 32 * i,
+                     p.a.dtype, sum == 0.0f ? 0.0f : o[i] / sum);
+    else
+      p.part_o[part_row * HD + lane + 32 * i] = o[i];
+  }
+  if (lane) return;
+  if (part_row >= 0)
+    p.part_nl[part_row] = make_float2(low, sum);
+  else if (p.lse)
+    p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = log2f(sum) - low;
 }
 
 // S^T of a tile. Few columns: two chains of products, so that one's latency hides the other's.
@@ -468,11 +537,6 @@ NRC_DEV Start find_start(const Plan& p, uint32_t hbs, uint32_t unit, uint32_t se
   return *found;
 }
 
-// A score's exponential is taken as 2^(s + ref): ref is LIFT less the largest score seen when the row's reference was last
-// set, and is set again (its sums rescaled) when an exponent passes LIFT + SLACK, so most tiles need no reduction over
-// their positions. f16 weights: up to 2^15, and with bits down to 2^-24, 2^-32 of the row's sum. UNSET: nothing seen.
-constexpr float SLACK = 7.0f, LIFT = 8.0f, UNSET = 3e38f;
-
 // Exponentials of 8 columns' scores, added to the rows' sums, as operand B of O^T.
 template <bool BF, int PARTS>
 NRC_DEV void weights_operand(uint32_t (&pb)[PARTS][2], const float (&s)[4], const float (&ref)[2], float (&l)[2]) {
@@ -500,9 +564,11 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
   __shared__ float n_s[WARPS][COLS], l_s[WARPS][COLS];
   __shared__ uint64_t warp_sums[WARPS];
   __shared__ Start start_s;
+  __shared__ uint32_t odd_s;  // columns whose sums are no numbers
   float(*o_s)[COLS][HD + 2] = reinterpret_cast<float(*)[COLS][HD + 2]>(dyn_s);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t hbs = p.a.kv.n_kv_heads * p.row_blocks;
+  if (threadIdx.x == 0) odd_s = 0;
   pdl_trigger();  // the join waits for this grid's end by itself
   Start st;
   if (p.direct) {
@@ -683,6 +749,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
         sum += f * l_s[w][col];
         o += f * o_s[w][col][d];
       }
+      if (fmaf(o, 0.0f, sum) != sum || !(sum < INFINITY)) atomicOr(&odd_s, 1u << col);  // NaN or infinite
       if (complete) {
         const uint32_t tok = r / p.gqa, head = h * p.gqa + r % p.gqa;
         store_from_f32(p.a.out, (int64_t)b * p.a.o_seq + (int64_t)tok * p.a.o_token + (int64_t)head * p.a.o_head + d,
@@ -692,6 +759,14 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
         p.part_o[((size_t)part * COLS + col) * HD + d] = o;
         if (d == 0) p.part_nl[(size_t)part * COLS + col] = make_float2(low, sum);
       }
+    }
+    __syncthreads();
+    if (odd_s) {
+      for (int c = warp; c < COLS; c += WARPS)
+        if ((odd_s >> c) & 1)
+          row_again<BF, HD>(p, b, h, rb * COLS + c, u0 * UNIT, u1 * UNIT, complete ? -1 : (int64_t)part * COLS + c);
+      __syncthreads();
+      if (threadIdx.x == 0) odd_s = 0;
     }
     // Work that starts here and goes on: the join kernel's item, with the number of blocks that hold its parts.
     if (u1 < units && !(first && u0) && threadIdx.x == 0) {

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
   constexpr uint32_t DRAIN = tc_drain(BF, PARTS), TMEM = WEIGHTS ? NP * 2 > 128 ? 256 : 128 : PARTS == 1 ? 256 : 512;  // two groups' scores, accumulators and sums
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[D], empty[D], s_full[2], s_empty[2], p_full[2], p_done[2], q_full, cut_full, drain;
-  __shared__ uint32_t tmem_s, dead;
+  __shared__ uint32_t tmem_s, dead, odd_s;  // odd_s: columns whose sums are no numbers
   static_assert(TC_MASKS >= D + 3, "the copies would overwrite the mask of a tile that is still to be read");
   __shared__ uint32_t cached_s[TC_MASKS][4];          // which positions of a tile are cached, by tile number
   __shared__ __align__(16) float fac_s[TC_COLS], ref_s[2][TC_COLS];  // factor of each row, its reference per group
@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     mbar_init(&cut_full, 1);
     mbar_init(&drain, 1);
     dead = 0;
+    odd_s = 0;
     fence_barrier_init();
     if (!WEIGHTS) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
@@ -653,6 +654,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         f_s[1][c] = f1;
         sum_s[c] = complete ? sum == 0.0f ? 0.0f : 1.0f / sum : 1.0f;
         if (r < p.rows) {
+          if (!(sum < INFINITY)) atomicOr(&odd_s, 1u << c);
           if (!complete)
             p.part_nl[(size_t)part * TC_COLS + c] = make_float2(low, sum);
           else if (p.lse)
@@ -694,6 +696,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             }
           }
         }
+        float zero = 0.0f;  // NaN where a sum is no number
+#pragma unroll
+        for (int k = 0; k < 16; k++) zero = fmaf(o[k], 0.0f, zero);
+        if (zero != 0.0f)
+#pragma unroll
+          for (int k = 0; k < 16; k++)
+            if (w.rb * TC_COLS + 16 * g + k < p.rows && !(fabsf(o[k]) < INFINITY)) atomicOr(&odd_s, 1u << (16 * g + k));
 #pragma unroll
         for (int k = 0; k < 16; k++) {
           const uint32_t c = 16 * g + k, r = w.rb * TC_COLS + c;
@@ -714,6 +723,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       }
       first = false;
       named_sync(3, TC_SOFTMAX);  // everything shared is read before the next piece writes it
+      if (odd_s) {
+        const uint32_t begin = min(w.u0 * p.tc_tile, w.seen), end = last ? w.len : min(w.u1 * p.tc_tile, w.seen);
+        for (int c = warp; c < TC_COLS; c += TC_SOFTMAX / 32)
+          if ((odd_s >> c) & 1)
+            row_again<BF, HD>(p, w.b, w.h, w.rb * TC_COLS + c, begin, end, complete ? -1 : (int64_t)part * TC_COLS + c);
+        named_sync(3, TC_SOFTMAX);
+        if (threadIdx.x == 0) odd_s = 0;
+      }
     }
   }
   tc_fence_before();

@@ -170,7 +170,7 @@ def run_odd(K, q, k, v, table, lens, scale):
     return out, w
 
 
-@pytest.mark.parametrize("case", [c for c in ODD if c[5] == c[6]], ids=lambda c: str(ODD.index(c)))
+@pytest.mark.parametrize("case", ODD, ids=[str(i) for i in range(len(ODD))])
 def test_infinite_keys_that_count_for_nothing(K, case):
     """Keys that are infinite where every query is below zero: their scores are -inf, their weights 0, and nothing else
     changes, whatever columns of a tile are no rows."""
@@ -186,3 +186,51 @@ def test_infinite_keys_that_count_for_nothing(K, case):
     out, w = run_odd(K, q, k, v, table, lens, 0.2)
     same(w, ww, wtol + 1e-30)
     same(out, want, tol)
+
+
+@pytest.mark.parametrize("case", ODD, ids=[str(i) for i in range(len(ODD))])
+def test_infinite_values_are_the_outputs(K, case):
+    """Infinite values, some at positions whose weight is far below a 16-bit number's: infinite outputs in their places, NaN
+    where both signs meet, everything else as it was; the weights do not change. One infinity is at the last position,
+    which only the last new token sees."""
+    q, k, v, table, lens = odd_case(K, case, 32)
+    for s, n in enumerate(lens.tolist()):
+        far = n // 2  # a key against the queries: a weight of about e^-40
+        mean = q[s].double().mean((0, 1))
+        R.put(k, table, s, far, (-mean / mean.norm() * 3).to(k.dtype).expand(k.shape[2], -1))
+        for t, at, x in ((3, 1, INF), (n // 3, 7, -INF), (far, 11, INF), (5, 20, INF), (n // 4, 20, -INF), (n - 1, 30, -INF),
+                         (n // 5, 9, NAN)):
+            row = R.rows(v, table, s, [t])[0].clone()
+            row[:, at] = x
+            R.put(v, table, s, t, row)
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.3)
+    out, w = run_odd(K, q, k, v, table, lens, 0.3)
+    same(w, ww, wtol + 1e-30)
+    same(out, want, tol)
+
+
+@pytest.mark.parametrize("case", ODD, ids=[str(i) for i in range(len(ODD))])
+def test_infinite_and_nan_keys_reach_their_rows_only(K, case):
+    """Keys of both signs of infinity and NaN: the rows that see a score of +inf or NaN are NaN, those of the other KV head,
+    the other sequence and the tokens before are not."""
+    q, k, v, table, lens = odd_case(K, case, 33)
+    n = int(lens[0])
+    for t, at, x in ((n - 2, 3, INF), (n - 1, 4, NAN), (n // 2, 6, -INF)):
+        row = R.rows(k, table, 0, [t])[0].clone()
+        row[1, at] = x
+        R.put(k, table, 0, t, row)
+    q[0, 0, :, 6] = q[0, 0, :, 6].abs() + 0.01  # the first token's scores at n // 2 are -inf
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.2)
+    out, w = run_odd(K, q, k, v, table, lens, 0.2)
+    same(out, want, tol)
+    same(w, ww, wtol + 1e-30)
+
+
+@pytest.mark.parametrize("case", [ODD[1], ODD[6]], ids=["few", "many"])
+def test_nan_queries_reach_their_rows_only(K, case):
+    q, k, v, table, lens = odd_case(K, case, 34)
+    q[0, 0, 1, 9] = NAN
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.2)
+    out, w = run_odd(K, q, k, v, table, lens, 0.2)
+    same(out, want, tol)
+    same(w, ww, wtol + 1e-30)
