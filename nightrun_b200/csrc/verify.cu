@@ -184,8 +184,10 @@ NRC_DEV uint32_t span_find(const Row<DT>& r, uint32_t t0, uint32_t t1, double be
   return (uint32_t)last;
 }
 
-// The span whose running sum first exceeds goal, and the running sum before it; where rounding leaves none, the last that
-// holds anything (before: -inf); -1 if none does. One warp; sums in index order, each lane `n / 32` of them.
+// The span that holds something and whose running sum first exceeds goal, and the running sum before it; where rounding
+// leaves none, the last that holds anything (before: -inf); -1 if none does. (A lane's running sum begins with the scan's, which
+// may be a rounding above the lane's before it: without the first condition a goal between the two would pick a span of
+// zeros.) One warp; sums in index order, each lane `n / 32` of them.
 NRC_DEV int pick_span(const double* sums, uint32_t n, double goal_of_total, double* total, double* before, int lane) {
   const uint32_t each = (n + 31) / 32, i0 = min(lane * each, n), i1 = min(i0 + each, n);
   double t = 0.0;
@@ -204,7 +206,7 @@ NRC_DEV int pick_span(const double* sums, uint32_t n, double goal_of_total, doub
   double at_over = 0.0;
   for (uint32_t i = i0; i < i1; i++) {
     const double v = sums[i];
-    if (over < 0 && at + v > goal) over = (int)i, at_over = at;
+    if (over < 0 && v > 0.0 && at + v > goal) over = (int)i, at_over = at;
     if (v > 0.0) last = (int)i;
     at += v;
   }
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 5 : 2) k_verify_draft
       if (lane >= o) run += y;
     }
     run += before;
-    const unsigned over = __ballot_sync(0xffffffffu, run > goal), some = __ballot_sync(0xffffffffu, f > 0.0);
+    const unsigned over = __ballot_sync(0xffffffffu, f > 0.0 && run > goal), some = __ballot_sync(0xffffffffu, f > 0.0);
     const int pick = over ? __ffs(over) - 1 : 31 - __clz(some);
     double at = __shfl_up_sync(0xffffffffu, run, 1);
     if (lane == 0) at = before;

@@ -234,3 +234,37 @@ def test_nan_queries_reach_their_rows_only(K, case):
     out, w = run_odd(K, q, k, v, table, lens, 0.2)
     same(out, want, tol)
     same(w, ww, wtol + 1e-30)
+
+
+# ------------------------------------------------------------------ drawn tokens
+
+
+@pytest.mark.parametrize("seqs", [16, 64])
+def test_drawn_tokens_hold_something_where_the_goal_meets_a_sum(K, seqs):
+    """The two halves of a row hold the same values in another order, spread over 70 binary orders, and u is a half: the goal
+    lies within a rounding of the sum over the first half, and zeros follow there. The drawn token has a probability, and
+    the sums before it and with it enclose the goal up to the roundings of 64-bit sums of 128 values (128 halves of a step)."""
+    import math
+
+    import numpy as np
+    vocab, drawn = 65536, 0
+    tokens, accepted = (torch.empty(seqs, *x, dtype=torch.int32, device="cuda") for x in ((1,), ()))
+    draft, u = torch.empty(seqs, 0, dtype=torch.int32, device="cuda"), torch.full((seqs, 1), 0.5, device="cuda")
+    for seed in range(384 // seqs):
+        r = np.random.default_rng(seed)
+        rows = np.zeros((seqs, 1, vocab), np.float32)
+        for s in range(seqs):
+            h = (r.random(64) * 2.0 ** -r.integers(0, 70, 64)).astype(np.float32)
+            w = r.permutation(h)
+            if s % 2:
+                w = np.concatenate([np.zeros(2, np.float32), np.delete(w, np.argsort(w)[:2])])
+            rows[s, 0, 511::512] = np.concatenate([h, w])
+        K.verify_draft(tokens, accepted, torch.from_numpy(rows).cuda(), None, draft, u)
+        for s, t in enumerate(tokens[:, 0].tolist()):
+            row = rows[s, 0].astype(np.float64)[511::512]
+            assert rows[s, 0, t] > 0, (seed, s, t)
+            i, goal = t // 512, math.fsum(row) / 2
+            slack = 128 * 2.0 ** -53 * math.fsum(row)
+            assert math.fsum(row[:i]) <= goal + slack and math.fsum(row[:i + 1]) >= goal - slack
+            drawn += 1
+    assert drawn == 384 and not accepted.any()
