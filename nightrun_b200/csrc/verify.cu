@@ -20,9 +20,9 @@ namespace cg = cooperative_groups;
 
 constexpr int VD_MAX_CLUSTER = 8;
 
-// What is left of p at one token: max(p - q, 0) after a refusal, p itself otherwise; NaN, infinities and negative values
-// count as nothing. The difference of two f32 values is formed in 64 bits.
-NRC_DEV double left_of(float p, float q) { return p > q && p <= FLT_MAX ? (double)p - (double)q : 0.0; }
+// What is left of p at one token: max(p - q, 0) after a refusal, p itself otherwise; NaN, infinities (of p or q) and negative
+// differences count as nothing. The difference of two f32 values is formed in 64 bits.
+NRC_DEV double left_of(float p, float q) { return p > q && fmaxf(p, -q) <= FLT_MAX ? (double)p - (double)q : 0.0; }
 
 // Two running sums of what is left.
 struct Sums {

@@ -268,3 +268,17 @@ def test_drawn_tokens_hold_something_where_the_goal_meets_a_sum(K, seqs):
             assert math.fsum(row[:i]) <= goal + slack and math.fsum(row[:i + 1]) >= goal - slack
             drawn += 1
     assert drawn == 384 and not accepted.any()
+
+
+def test_draft_probabilities_below_every_number_count_as_nothing(K):
+    """A draft distribution that holds -inf or NaN at a token: nothing is left there, as with any infinity."""
+    vocab = 3000
+    p = torch.zeros(3, 2, vocab)
+    p[:, 0, 100:200] = 0.01
+    q = torch.zeros(3, 1, vocab)
+    q[:, 0, 7], q[0, 0, 150], q[1, 0, 2000], q[2, 0, 150] = 1.0, -INF, -INF, NAN
+    tokens, accepted = torch.empty(3, 2, dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    u = torch.tensor([[0.5, 0.501], [0.5, 0.501], [0.5, 0.501]])
+    K.verify_draft(tokens, accepted, p.cuda(), q.cuda(), torch.full((3, 1), 7, dtype=torch.int32, device="cuda"), u.cuda())
+    # What is left: 100 tokens of 0.01 less the odd one; the goal 0.501 of the sum lies in the 50th or the 51st of them.
+    assert accepted.tolist() == [0, 0, 0] and tokens.tolist() == [[149, -1], [150, -1], [149, -1]]
