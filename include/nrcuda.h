@@ -159,7 +159,9 @@ int nrc_rope_apply(float* x, size_t len, size_t head_dim, const float* freqs_hos
 /* Pages of K and V rows: the row of (page, offset, head) is head_dim contiguous values at
  * page * page_stride + offset * pos_stride + head * head_stride, in k and in v alike. The position
  * `slot` of sequence s lies in page table[s * table_stride + slot / page_size] at offset
- * slot % page_size. k, v and the strides are multiples of 16 bytes; head_dim is 32, 64, 96 or 128. */
+ * slot % page_size. k, v and the strides are multiples of 16 bytes; head_dim is 32, 64, 96 or 128. Rows lie apart, and K's from
+ * V's where a call writes them. What a call writes and what else it takes lie apart too, but for the in-place forms that it
+ * names: tensors that overlap are refused, interleaved ones that do not are taken. */
 typedef struct nrc_paged_kv {
   void* k;
   void* v;
@@ -182,7 +184,7 @@ int nrc_rope_freqs_yarn(float* out_host, float* mscale, size_t rot_dim, float th
  * (style 0: values 2i, 2i+1; style 1: i, i + rot_dim/2; values from rot_dim on pass unchanged)
  *   (a, b) -> mscale * (a cos - b sin, a sin + b cos),  angle = pos[t] * freqs[i],
  * the angle in 64 bits and the rest in f32, rounded once to the output's type (nearest even). q goes
- * to q_out (q itself is allowed), k and v to slot[t] of sequence seq[t] (slot < 0: not cached).
+ * to q_out (q itself, with its strides, is allowed), k and v to slot[t] of sequence seq[t] (slot < 0: not cached).
  * q, q_out: [tokens][n_heads][head_dim], k and v: [tokens][kv heads][head_dim], of `dtype`; pos, seq,
  * slot: int32 [tokens]. No two tokens of a call share (seq, slot). */
 typedef struct nrc_rope_args {
@@ -248,7 +250,7 @@ int nrc_kv_evict(const nrc_paged_kv* kv, int32_t* kept, int32_t* new_lens, float
  * when every draft was taken, from p_a: the first index whose running sum, in 64 bits, exceeds
  * u[n_max] times the whole sum (p_a itself where the difference leaves nothing; token 0 where that
  * holds nothing positive either; NaN and infinities count as nothing). tokens[s] = the a taken drafts, the drawn
- * token, then -1; accepted[s] = a. p: [n_seqs][n_max + 1][vocab], q: [n_seqs][n_max][vocab] (NULL:
+ * token, then -1; accepted[s] = a; accepted == n_draft is allowed, and for one sequence tokens == draft. p: [n_seqs][n_max + 1][vocab], q: [n_seqs][n_max][vocab] (NULL:
  * each draft was certain, q = 1 at it), of `dtype`, with sequence and token strides; draft: int32
  * [n_seqs][n_max] (an id outside the vocabulary is refused); u: f32 [n_seqs][n_max + 1] in [0, 1);
  * n_draft: int32 [n_seqs] or NULL (n_max everywhere); tokens: int32 [n_seqs][n_max + 1]. */

@@ -4,8 +4,10 @@ over a paged KV cache"). Re-exported by `kernels`, with its conventions:
 outputs first, asynchronous on the current torch stream (or `stream=`).
 
 Where the tensors live on another device than the current one, the call is
-made on theirs. Shapes, types, strides and devices that do not fit raise
-NrcError (INVALID); tensors that are not on a GPU raise ValueError.
+made on theirs. Shapes, types, strides and devices that do not fit, and
+outputs that overlap one another or an input (but for the in-place forms
+named below), raise NrcError (INVALID); tensors that are not on a GPU raise
+ValueError.
 """
 import ctypes as C
 import struct
@@ -89,13 +91,13 @@ class PagedKV:
         _need(self.page_size > 0 and self.n_kv_heads > 0, "empty pages")
         _need(not any(x % 8 for x in (ps, rs, hs)) and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0,
               "pages and their strides must be multiples of 16 bytes")
-        _need(not any(n > 1 and x == 0 for n, x in zip(k_pages.shape, k_pages.stride())), "rows of the pages overlap")
         _need(self.n_pages < 2 ** 31 and self.max_pages * self.page_size < 2 ** 31 and self.n_seqs < 65536
               and self.n_kv_heads <= 16384, "cache too large")
         self.desc = PagedKVDesc(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), self.n_pages, ps, rs, hs,
                                 self.page_size, self.n_kv_heads, self.head_dim, self.n_seqs, self.max_pages,
                                 table.stride(0) if self.n_seqs > 1 else self.max_pages, _DTYPES[k_pages.dtype])
         self._ref = C.byref(self.desc)
+        check(lib().nrc_attn_paged_workspace(self._ref, 1, self.n_kv_heads, 0, 0, C.byref(C.c_size_t())))  # rows that overlap
 
 
 def rope_freqs_yarn(rot_dim, theta, factor, original_context, beta_fast=32.0, beta_slow=1.0):
@@ -223,7 +225,8 @@ def verify_draft(tokens, accepted, p, q, draft, u, n_draft=None, stream=None):
     (None: each draft was certain), draft int32 [seqs, n], u float32 [seqs, n + 1] in [0, 1), n_draft
     int32 [seqs] (None: n). Draft i is taken while u[i] * q_i(draft) < p_i(draft); the token after the
     taken ones is drawn with u[n] from max(p - q, 0) at a refusal, else from p. tokens int32
-    [seqs, n + 1]: taken drafts, the drawn token, -1; accepted int32 [seqs]: how many were taken."""
+    [seqs, n + 1]: taken drafts, the drawn token, -1; accepted int32 [seqs]: how many were taken. accepted
+    may be n_draft, and for one sequence tokens may begin where draft does."""
     i, dt = p.get_device(), p.dtype
     if i < 0 or not i == tokens.get_device() == accepted.get_device() == draft.get_device() == u.get_device():
         _elsewhere(p.device, p, tokens, accepted, draft, u)

@@ -282,3 +282,50 @@ def test_draft_probabilities_below_every_number_count_as_nothing(K):
     K.verify_draft(tokens, accepted, p.cuda(), q.cuda(), torch.full((3, 1), 7, dtype=torch.int32, device="cuda"), u.cuda())
     # What is left: 100 tokens of 0.01 less the odd one; the goal 0.501 of the sum lies in the 50th or the 51st of them.
     assert accepted.tolist() == [0, 0, 0] and tokens.tolist() == [[149, -1], [150, -1], [149, -1]]
+
+
+# ------------------------------------------------------------------ tensors beside one another
+
+
+def test_interleaved_and_in_place_tensors(K):
+    """What lies between one another's rows without touching them is taken, and so are the in-place forms: q, k, v and q's
+    output in one projection, queries and outputs in alternate rows, K's and V's pages in turn, drafts in the tokens' place."""
+    g = gen(3)
+    hq, hk, d, page = 4, 2, 64, 8
+    lens = torch.tensor([33, 20], dtype=torch.int32)
+    both = torch.randn(12, 2, page, hk, d, generator=g).to(F16)
+    table = torch.randperm(12, generator=g)[:10].view(2, 5).int()
+    gb = both.cuda()
+    kv = K.PagedKV(gb[:, 0], gb[:, 1], table.cuda())
+    x = torch.randn(2, hq + 2 * hk, d, generator=g)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    freqs = torch.tensor(K.rope_freqs(d, 10000.0), device="cuda")
+    gx = x.cuda()
+    K.rope_append(gx[:, :hq], gx[:, :hq], gx[:, hq:hq + hk], gx[:, hq + hk:], kv, freqs, i32(32, 19), i32(0, 1), i32(32, 19))
+    pos = torch.tensor([32, 19])
+    want = R.rope(x[:, :hq], pos, freqs.cpu(), 1, 1.0)
+    assert bool(((gx[:, :hq].double().cpu() - want).abs() <= R.rope_tolerance(x[:, :hq], freqs.cpu(), 1, 1.0, F32, want)).all())
+    assert torch.equal(gx[:, hq:].cpu(), x[:, hq:])
+    both = gb.cpu()
+    for s, t in ((0, 32), (1, 19)):
+        assert torch.equal(R.rows(both[:, 1], table, s, [t])[0], x[s, hq + hk:].to(F16))
+    pair = torch.zeros(2, 1, hq, 2, d, device="cuda")  # a head's queries, then its output
+    pair[:, :, :, 0] = gx[:, None, :hq]
+    K.attn_paged(pair[:, :, :, 1], pair[:, :, :, 0], kv, lens.cuda(), 0.125)
+    want, _, size, big = R.attention(gx[:, None, :hq].cpu(), both[:, 0], both[:, 1], table, lens, 0.125)
+    tol, _ = R.attention_tolerance(F32, F16, d, 33, size, big, want)
+    assert bool(((pair[:, :, :, 1].double().cpu() - want).abs() <= tol).all())
+    p = torch.rand(1, 4, 500, generator=g)
+    q, u = torch.rand(1, 3, 500, generator=g), torch.rand(1, 4, generator=g)
+    draft = torch.randint(0, 500, (1, 3), generator=g, dtype=torch.int32)
+    tokens = torch.cat([draft, draft[:, :1]], 1).cuda()
+    number = i32(2)
+    K.verify_draft(tokens, number, p.cuda(), q.cuda(), tokens[:, :3], u.cuda(), number)
+    want_t, want_a = R.verify(p, q, draft, u, torch.tensor([2]))
+    assert torch.equal(tokens.cpu(), want_t) and torch.equal(number.cpu(), want_a)
+    shifted = gb.view(-1).as_strided((11, page, hk, d), gb[:, 0].stride(), 8)  # V's rows 16 bytes behind K's
+    one_pool = K.PagedKV(gb[:11, 0], shifted, table.cuda() % 11)
+    with pytest.raises(NrcError):
+        K.rope_append(gx[:, :hq], gx[:, :hq], gx[:, hq:hq + hk], gx[:, hq + hk:], one_pool, freqs, i32(1, 1), i32(0, 1), i32(1, 1))
+    with pytest.raises(NrcError):
+        K.PagedKV(*(gb[:, i].as_strided(gb[:, i].shape, (gb.stride(0), gb.stride(2), 32, 1)) for i in (0, 1)), table.cuda())
