@@ -160,8 +160,9 @@ int nrc_rope_apply(float* x, size_t len, size_t head_dim, const float* freqs_hos
  * page * page_stride + offset * pos_stride + head * head_stride, in k and in v alike. The position
  * `slot` of sequence s lies in page table[s * table_stride + slot / page_size] at offset
  * slot % page_size. k, v and the strides are multiples of 16 bytes; head_dim is 32, 64, 96 or 128. Rows lie apart, and K's from
- * V's where a call writes them. What a call writes and what else it takes lie apart too, but for the in-place forms that it
- * names: tensors that overlap are refused, interleaved ones that do not are taken. */
+ * V's where a call writes them. Outputs lie apart from one another and from the call's inputs, but for the in-place forms that it
+ * names: queries, outputs, weights, workspaces, lengths and tokens that overlap are refused, interleaved ones that do not
+ * are taken. */
 typedef struct nrc_paged_kv {
   void* k;
   void* v;

@@ -261,7 +261,12 @@ int nrc_attn_paged(const nrc_paged_kv* kv, const nrc_attn_args* r, void* stream)
   if (need && (!r->workspace || r->workspace_bytes < need || !aligned16(r->workspace)))
     return nrc_fail_api(NRC_ERR_INVALID, "workspace of %llu bytes, 16-byte aligned: %zu needed",
                         r->workspace ? (unsigned long long)r->workspace_bytes : 0ull, need);
-  if (overlap(out, rows(r->q, r->q_seq, r->q_token, r->q_head))) return overlapping("out and q");  // q is read again for the weights
+  const Rows q = rows(r->q, r->q_seq, r->q_token, r->q_head), lens = flat(r->lens, kv->n_seqs * 4ull),
+             w = flat(r->weights, (uint64_t)kv->n_seqs * kv->n_kv_heads * r->weights_len * 4), ws = flat(need ? r->workspace : nullptr, need);
+  if (overlap(out, q)) return overlapping("out and q");  // q is read again for the weights
+  for (const Rows& x : {out, q, lens})
+    if (overlap(w, x) || overlap(ws, x) || overlap(ws, w)) return overlapping("weights or workspace and the other tensors");
+  if (overlap(out, lens)) return overlapping("out and lens");
   return cuda_rc(paged_attn_run(a, static_cast<cudaStream_t>(stream)), "attn_paged");
 }
 

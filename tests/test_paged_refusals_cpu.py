@@ -93,6 +93,10 @@ def test_attn_paged_outputs_that_overlap(L):
                dict(out=(at, 256, 256, 64), q=(at - 2 * 256 * 4, 256, 256, 64)),
                dict(out=(at, 256, 256, 64), q=(at + 63 * 4, 512, 512, 128))):
         assert said(L, attn(L, desc(), **kw), "overlap"), kw
+    w = dict(weights=FAKE << 5, wlen=32)
+    for kw in (dict(weights=at + 64), dict(weights=(FAKE << 4) - 4), dict(weights=(FAKE << 9) - 8), dict(ws=FAKE << 5), dict(ws=at),
+               dict(ws=FAKE << 9), dict(lens=at + 1020)):
+        assert said(L, attn(L, desc(), **{**w, **kw}), "overlap"), kw
 
 
 def test_evict_tensors_that_overlap(L):
