@@ -213,8 +213,9 @@ int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* args, void* str
  *   out = sum_t p_t V_t,  p = softmax(scale * q . K_t),
  * infinite keys and values as in f32: a score of -inf has weight 0, one of +inf or NaN makes its row NaN, an infinite value of
  * weight above 0 is the output's; rows that do not see them are unharmed (they cost such a row a slower pass);
- * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into as
- * many cache-typed parts as hold all the bits of `dtype`. q and out: [n_seqs][n_new][n_heads]
+ * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into parts of the cache's type. q
+ * whole, but f32 over f16 in 22 bits below its row's largest value; p in 22 bits (f16) or 16 (bf16; f32 calls 24), however wide
+ * out is. q and out: [n_seqs][n_new][n_heads]
  * [head_dim] of `dtype`, apart from each other; lens: int32 [n_seqs]. weights (or NULL): f32 [n_seqs][kv heads][weights_len];
  * the weight that a position received from all the query heads of the KV head and all new tokens is
  * added to it. max_len: no sequence is longer (0: the table's width). workspace:

@@ -30,10 +30,12 @@
 // memory. Measured: 64 sequences of 4096, 32/8 heads of 128, bf16: 174 us, 6.2 TB/s (0.95 of measured); 64 ragged ones up to
 // 16384: 158 us (0.96); one of 131072: 88 us and the join 8 us more (0.86).
 //
-// Split parts. The tensor cores take operands of the cache's type. q (scaled by a power of two to at most 2 per row) and
-// p enter as PARTS values of that type whose sum holds the bits that the output's type can show: one where the output is
-// no wider than the cache, two f16 (22 bits) or three bf16 (24 bits) for f32, two bf16 for f16. Products of the parts go to
-// the same f32 accumulators.
+// Split parts. The tensor cores take operands of the cache's type. q (scaled by a power of two to at most 2 per row) enters
+// as PARTS values of that type whose sum holds its bits: one where it is no wider than the cache, two bf16 for f16, three
+// bf16 for f32 (24 bits), two f16 for f32 (22 bits, of a row's largest value: f16's smallest step ends them 2^-25 below
+// it). The weights p enter in as many, two at least (16 or 22 bits): in one part each weight would be rounded to the output's own
+// width and the output be some 30% further off (f16: 2.5e-4 instead of 2.1e-4 of it, bf16: 2.1e-3 instead of 1.7e-3); the
+// second costs 1 to 4% (bf16: 64 sequences of 4096 169 and 170 us, 16 with 8 new tokens on tcgen05 84 and 88 us). Products of the parts go to the same f32 accumulators.
 #pragma once
 #include "paged.cuh"
 #include "tma.cuh"
@@ -107,6 +109,7 @@ NRC_DEV uint32_t pack2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+constexpr int weight_parts(int parts) { return parts < 2 ? 2 : parts; }
 template <bool BF>
 NRC_DEV float2 unpack2(uint32_t x) {
   if (BF) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
@@ -558,7 +561,7 @@ NRC_DEV void weights_operand(uint32_t (&pb)[PARTS][2], const float (&s)[4], cons
 
 template <bool BF, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid_constant__ Plan p) {
-  constexpr int MT = HD / 16, COLS = 8 * NT;
+  constexpr int MT = HD / 16, COLS = 8 * NT, WP = weight_parts(PARTS);
   extern __shared__ __align__(16) uint8_t dyn_s[];  // the warps' sums, to be joined
   __shared__ Queries<HD, PARTS, NT> qs;
   __shared__ float n_s[WARPS][COLS], l_s[WARPS][COLS];
@@ -675,13 +678,13 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
         for (int j = 0; j < MT; j++) v.operand(a[j], j);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          uint32_t pb[PARTS][2];
-          weights_operand<BF, PARTS>(pb, s[n], ref[n], l[n]);
+          uint32_t pb[WP][2];
+          weights_operand<BF, WP>(pb, s[n], ref[n], l[n]);
 #pragma unroll
           for (int j = 0; j < MT; j++) {
             float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < PARTS; i++) mma<BF>(d, a[j], pb[i][0], pb[i][1]);
+            for (int i = 0; i < WP; i++) mma<BF>(d, a[j], pb[i][0], pb[i][1]);
             add4(acc[j][n], d);
           }
         }
@@ -690,8 +693,8 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
         const uint32_t tok0 = rb * COLS / p.gqa, tok1 = min(p.a.n_new, (rb * COLS + COLS - 1) / p.gqa + 1);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          uint32_t pb[PARTS][2];
-          weights_operand<BF, PARTS>(pb, s[n], ref[n], l[n]);
+          uint32_t pb[WP][2];
+          weights_operand<BF, WP>(pb, s[n], ref[n], l[n]);
           for (uint32_t tok = tok0; tok < tok1; tok++) {
             const uint32_t behind = p.a.n_new - 1 - tok, stop = len > behind ? len - behind : 0, at = p0 + 2 * t;
             const uint32_t mask0 = (at < stop ? 0xffffu : 0u) | (at + 1 < stop ? 0xffff0000u : 0u);
@@ -703,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, resident(HD, NT)) k_attn(const __grid
               a[0] &= mask0, a[1] &= mask0, a[2] &= mask1, a[3] &= mask1;
               float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int i = 0; i < PARTS; i++) mma<BF>(d, a, pb[i][0], pb[i][1]);
+              for (int i = 0; i < WP; i++) mma<BF>(d, a, pb[i][0], pb[i][1]);
 #pragma unroll
               for (int i = 0; i < 4; i++)
                 if ((rb * COLS + 8 * n + 2 * t + (i & 1)) / p.gqa == tok) acc[j][n][i] += d[i];

@@ -50,7 +50,7 @@ constexpr int TC_COLS = 32, TC_THREADS = 10 * 32, TC_SOFTMAX = 256;
 constexpr int tc_half(int hd) { return TC_TILE * hd * 2; }  // bytes of a half stage: one tile of K or V
 constexpr int tc_ring(int hd, int parts) { return hd == 64 ? 6 : parts < 3 ? 5 : 4; }
 constexpr int tc_smem(int hd, int parts, bool weights) {
-  return tc_ring(hd, parts) * tc_half(hd) + (weights ? 0 : 2 * parts * TC_TILE * 64) + parts * TC_COLS * hd * 2 + 1024;
+  return tc_ring(hd, parts) * tc_half(hd) + (weights ? 0 : 2 * weight_parts(parts) * TC_TILE * 64) + parts * TC_COLS * hd * 2 + 1024;
 }
 
 NRC_DEV void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
@@ -155,8 +155,10 @@ NRC_DEV bool next_work(const Plan& p, Start& st, uint32_t hbs, uint32_t setup, W
 // added over the columns by the thread that owns the position.
 template <bool BF, int HD, int PARTS, bool WEIGHTS>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ Plan p) {
-  constexpr int D = tc_ring(HD, PARTS), HALF = tc_half(HD), PB = TC_TILE * 64, NP = TC_COLS * PARTS;
-  constexpr uint32_t DRAIN = tc_drain(BF, PARTS), TMEM = WEIGHTS ? NP * 2 > 128 ? 256 : 128 : PARTS == 1 ? 256 : 512;  // two groups' scores, accumulators and sums
+  constexpr int D = tc_ring(HD, PARTS), HALF = tc_half(HD), PB = TC_TILE * 64;
+  constexpr int WP = weight_parts(PARTS), NP = TC_COLS * PARTS, NW = TC_COLS * WP;  // columns of S and of O: a part after the other
+  constexpr uint32_t DRAIN = tc_drain(BF, PARTS), TMEM = WEIGHTS ? NP * 2 > 128 ? 256 : 128 : PARTS == 1 ? 256 : 512;
+  static_assert(2 * NP + (WEIGHTS ? 0 : 2 * NW + 2 * TC_COLS) <= TMEM, "two groups' scores, accumulators and sums");
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[D], empty[D], s_full[2], s_empty[2], p_full[2], p_done[2], q_full, cut_full, drain;
   __shared__ uint32_t tmem_s, dead, odd_s;  // odd_s: columns whose sums are no numbers
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t hbs = p.a.kv.n_kv_heads * (WEIGHTS ? 1 : p.row_blocks), setup = WEIGHTS ? TC_WEIGHTS_SETUP : TC_SETUP;
   const uint32_t base = (smem_u32(dyn) + 1023) & ~1023u;
-  const uint32_t ring = base, p_buf = ring + D * HALF, q_buf = p_buf + (WEIGHTS ? 0 : 2 * PARTS * PB);
+  const uint32_t ring = base, p_buf = ring + D * HALF, q_buf = p_buf + (WEIGHTS ? 0 : 2 * WP * PB);
   if (!WEIGHTS) pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < D; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -312,9 +314,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
     uint32_t item = 0, used[2] = {0, 0}, works = 0;
     bool ok = true;
-    const uint32_t id_s = idesc_f16(BF, NP, false, false), id_o = idesc_f16(BF, NP, true, true);
+    const uint32_t id_s = idesc_f16(BF, NP, false, false), id_o = idesc_f16(BF, NW, true, true);
     const Desc q_desc = swizzled_desc(q_buf, 16, 1024, 2), p_desc0 = swizzled_desc(p_buf, PB, 512, 4),
-               p_desc1 = swizzled_desc(p_buf + PARTS * PB, PB, 512, 4);
+               p_desc1 = swizzled_desc(p_buf + WP * PB, PB, 512, 4);
     auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
     while (ok && next_work<WEIGHTS>(p, st, hbs, setup, w)) {
       if (w.tiles == 0) continue;  // nor do the softmax warps arrive
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           tc_fence_after();
           const Desc a = swizzled_desc(ring + slot * HALF, HD == 64 ? 0 : TC_TILE * 128, 1024, 2);
           const Desc b = g ? p_desc1 : p_desc0;
-          const uint32_t d = tmem + (2 + g) * NP, onto = (i - 1) / 2 % DRAIN;
+          const uint32_t d = tmem + 2 * NP + g * NW, onto = (i - 1) / 2 % DRAIN;
           if (leader) {
 #pragma unroll
             for (int s = 0; s < TC_TILE / 16; s++) tc_mma_f16(d, a.at(s * 2048), b.at(s * 1024), id_o, s ? 1u : onto);
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     // ---------------------------------------------------------------- softmax
     const int g = warp >> 2, quarter = warp & 3, row = threadIdx.x & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_tm = lane_base + g * NP, o_tm = lane_base + 2 * NP, sum_tm = lane_base + 4 * NP + g * TC_COLS;
+    const uint32_t s_tm = lane_base + g * NP, o_tm = lane_base + 2 * NP, sum_tm = lane_base + 2 * NP + 2 * NW + g * TC_COLS;
     uint32_t used = 0, tile = 0;
     bool ok = true, first = true;
     if (WEIGHTS) pdl_wait();  // the sums below are the kernels' before
@@ -448,8 +450,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
 #pragma unroll
           for (int c = 0; c < 16; c++) sum[c] = used - used0 > DRAIN ? sum[c] : 0u;  // the first time nothing stands there
 #pragma unroll
-          for (int j = 0; j < PARTS; j++) {
-            tc_ld16(o_tm + g * NP + j * TC_COLS + 16 * h, o);
+          for (int j = 0; j < WP; j++) {
+            tc_ld16(o_tm + g * NW + j * TC_COLS + 16 * h, o);
             tc_wait_ld_regs<16>(o);
 #pragma unroll
             for (int c = 0; c < 16; c += 2) {
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             tc_fence_after();
             if (ok) {
 #pragma unroll
-              for (int j = 0; j < PARTS; j++) scaled(o_tm + g * NP + j * TC_COLS);
+              for (int j = 0; j < WP; j++) scaled(o_tm + g * NW + j * TC_COLS);
               if (used - used0 > DRAIN) scaled(sum_tm);
               tc_wait_st();
             }
@@ -578,18 +580,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         }
         if (used) ok = __all_sync(0xffffffffu, ok && wait(&p_done[g], (used - 1) & 1));  // the weights before are used up
         if (ok && used != used0 && (used - used0) % DRAIN == 0) drained(sum_tm);
-        const uint32_t p_row = p_buf + g * PARTS * PB + row * 64;
+        const uint32_t p_row = p_buf + g * WP * PB + row * 64;
 #pragma unroll
         for (int c0 = 0; c0 < TC_COLS / 2; c0 += 4) {
-          uint32_t v[4][PARTS];
+          uint32_t v[4][WP];
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             const float2 e = make_float2(exp2_fast(x[c0 + c].x), exp2_fast(x[c0 + c].y));
             l[c0 + c] = __fadd2_rn(l[c0 + c], e);
-            split2<BF, PARTS>(e.x, e.y, v[c]);
+            split2<BF, WP>(e.x, e.y, v[c]);
           }
 #pragma unroll
-          for (int j = 0; j < PARTS; j++)
+          for (int j = 0; j < WP; j++)
             st_shared16(p_row + j * PB + (((c0 / 4) ^ ((row >> 1) & 3)) << 4), v[0][j], v[1][j], v[2][j], v[3][j]);
         }
         fence_proxy_async_smem();
@@ -600,7 +602,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       tile += w.tiles;
       if (!WEIGHTS && used != used0) {  // the whole sums to the accumulator's first columns, where both groups read them
         ok = __all_sync(0xffffffffu, ok && wait(&p_done[g], (used - 1) & 1));
-        if (ok) drained(o_tm + g * NP);
+        if (ok) drained(o_tm + g * NW);
       }
       tc_fence_before();
       // Sums over the positions: lanes, then (below) warps and groups.
@@ -672,7 +674,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       for (int h = 0; h < 2; h++) {  // the groups' sums
         if (h ? !have1 : !have0) continue;
         uint32_t v[16];
-        tc_ld16(o_tm + h * NP + 16 * g, v);
+        tc_ld16(o_tm + h * NW + 16 * g, v);
         tc_wait_ld_regs<16>(v);
 #pragma unroll
         for (int k = 0; k < 16; k++) o[k] = fmaf(f_s[h][16 * g + k], __uint_as_float(v[k]), o[k]);

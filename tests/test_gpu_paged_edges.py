@@ -103,13 +103,15 @@ def expected(q, k_pages, v_pages, table, lens, scale):
     leaves NaN in its row, an infinite value at a position of weight above 0 is the output's.
 
     Scores: d products, summed in f32 one after the other at worst, (d + 8) 2^-24 of the sum of magnitudes, and operands
-    that hold 2^-22 of theirs; weights and sums as in R.attention_tolerance."""
+    that hold 2^-22 of theirs. Weights enter in two parts of the cache's type at least: two roundings of 2^-11 or 2^-8, and
+    f16's smallest step, 2^-25 off where the row's sum is 2^8 or more. Sums as in R.attention_tolerance, but that tcgen05 adds
+    128 tile sums of 16-bit calls, cut by 2^-23 each, before one to nearest: 2^-16."""
     b, n, hq, d = q.shape
     hk, slots = k_pages.shape[2], table.shape[1] * k_pages.shape[1]
     g = hq // hk
     out, tol = torch.zeros(b, n, hq, d, dtype=torch.float64), torch.zeros(b, n, hq, d, dtype=torch.float64)
     weights, wtol = torch.zeros(b, hk, slots, dtype=torch.float64), torch.zeros(b, hk, slots, dtype=torch.float64)
-    enter = 2.0 ** -22 if q.dtype == F32 else 2.0 ** -16 if R.HALF[q.dtype] < R.HALF[k_pages.dtype] else R.HALF[k_pages.dtype]
+    enter = 2.0 ** -22 if q.dtype == F32 or k_pages.dtype == F16 else 2.0 ** -16  # f32: three parts over bf16; else two
     for s in range(b):
         m = int(lens[s])
         keys, values = (R.rows(x, table, s, range(m)).double() for x in (k_pages, v_pages))
@@ -126,7 +128,8 @@ def expected(q, k_pages, v_pages, table, lens, scale):
                 delta = big * ((d + 8) * 2.0 ** -24 + 2.0 ** -22)
                 sums = (3 * sees / 16 + 40) * 2.0 ** -23
                 size = (p[:, None] * vv.abs()).nan_to_num(0.0, 0.0, 0.0).sum(0)
-                tol[s, j, h] = (size * (2.2 * delta + enter + 2.0 ** -20 + 2 * sums)
+                enters = enter + sees * 2.0 ** -33 + (0 if q.dtype == F32 else 2.0 ** -16)
+                tol[s, j, h] = (size * (2.2 * delta + enters + 2.0 ** -20 + 2 * sums)
                                 + out[s, j, h].abs().nan_to_num(0.0, 0.0, 0.0) * R.HALF[q.dtype] + R.TINY[q.dtype])
                 weights[s, h // g, :sees] += p
                 wtol[s, h // g, :sees] += p * (2.2 * delta + 2.0 ** -20 + sums + 2.0 ** -21)
@@ -168,6 +171,22 @@ def run_odd(K, q, k, v, table, lens, scale):
     K.attn_paged(alone, q.cuda(), kv, lens.cuda(), scale)
     assert torch.equal(alone.isnan(), out.isnan()) and torch.equal(alone.nan_to_num(7.0), out.nan_to_num(7.0))
     return out, w
+
+
+FINE = [c for c in ODD if c[5] != F32] + [
+    ([2, 3, 5], 1, 8, 2, 64, F16, F16, 16), ([2, 3, 5], 1, 8, 2, 128, BF16, BF16, 16), ([900, 40], 1, 8, 2, 64, BF16, F16, 16),
+    ([900, 40], 1, 24, 2, 64, BF16, BF16, 7), ([500, 333], 5, 8, 2, 64, BF16, BF16, 16), ([500, 333], 5, 8, 2, 128, F16, F16, 16)]
+
+
+@pytest.mark.parametrize("case", FINE, ids=[str(i) for i in range(len(FINE))])
+def test_16_bit_outputs_are_rounded_once(K, case):
+    """16-bit outputs against 64 bits: the output's own rounding, and next to it only what two parts of a weight leave (one
+    part would add a rounding of the cache's type to every weight)."""
+    q, k, v, table, lens = odd_case(K, case, 35)
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.3)
+    out, w = run_odd(K, q, k, v, table, lens, 0.3)
+    same(out, want, tol)
+    same(w, ww, wtol + 1e-30)
 
 
 @pytest.mark.parametrize("case", ODD, ids=[str(i) for i in range(len(ODD))])
