@@ -48,6 +48,14 @@ def _ints(t, shape, what):
         raise NrcError(NRC_ERR_INVALID, f"{what}: contiguous int32 of shape {tuple(shape)}")
 
 
+def _on(index, fn, *args):
+    """fn(*args) with device `index` the current one."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def _call(device, stream, fn, *args):
     """fn(*args, stream) on `device` and `stream` (None: the device's current one)."""
     index = device.index
@@ -56,11 +64,7 @@ def _call(device, stream, fn, *args):
         handle = stream.cuda_stream
     else:
         handle = torch._C._cuda_getCurrentRawStream(index)  # current_stream() takes 3 us to wrap it
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, handle)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, handle)
+    rc = _on(index, fn, *args, handle)
     if rc:
         check(rc)
 
@@ -141,8 +145,8 @@ def attn_paged_workspace(q, kv, weights=False, max_len=0):
     """The workspace of attn_paged calls of this shape: keep it, and use it in one call at a time."""
     _need(q.dim() in (3, 4), "q: [seqs, new, heads, head_dim] or [seqs, heads, head_dim]")
     need = C.c_size_t()
-    check(lib().nrc_attn_paged_workspace(kv._ref, q.shape[1] if q.dim() == 4 else 1, q.shape[-2], int(weights), max_len,
-                                         C.byref(need)))
+    check(_on(kv.index, lib().nrc_attn_paged_workspace, kv._ref, q.shape[1] if q.dim() == 4 else 1, q.shape[-2], int(weights),
+              max_len, C.byref(need)))  # its size goes by the device's SMs
     return torch.empty(need.value, dtype=torch.uint8, device=kv.device)
 
 

@@ -139,3 +139,32 @@ def test_workspaces_that_do_not_fit(L, with_weights, new):
     assert need(max_len=200) < need() and need(weights=1) > need(weights=0)
     if with_weights:
         assert said(L, attn(L, desc(**BIG), **{**kw, "wsb": need(weights=0)}), "workspace")
+
+
+def test_the_workspace_is_sized_for_the_tensors_device(monkeypatch):
+    """Its size goes by the number of SMs: asked for on the device of the pages, whatever the current one is."""
+    import torch
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def nrc_attn_paged_workspace(self, ref, new, heads, weights, max_len, out):
+            seen.append((current[0], new, heads, weights))
+            out._obj.value = 512
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(paged, "lib", Lib)
+    kv = type("KV", (), dict(index=1, _ref=None, device=torch.device("cpu")))()
+    assert paged.attn_paged_workspace(torch.empty(2, 3, 4, 64), kv, weights=True).nbytes == 512
+    assert seen == [(1, 3, 4, 1)] and current == [0]
