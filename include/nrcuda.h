@@ -218,7 +218,8 @@ int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* args, void* str
  * out is. q and out: [n_seqs][n_new][n_heads]
  * [head_dim] of `dtype`, apart from each other; lens: int32 [n_seqs]. weights (or NULL): f32 [n_seqs][kv heads][weights_len];
  * the weight that a position received from all the query heads of the KV head and all new tokens is
- * added to it. max_len: no sequence is longer (0: the table's width). workspace:
+ * added to it. max_len: no sequence is longer (0: the table's width); one that is, or is longer than weights_len, is cut there and
+ * reported. workspace:
  * nrc_attn_paged_workspace bytes, 16-byte aligned, used by one call at a time. */
 typedef struct nrc_attn_args {
   void* out;

@@ -77,6 +77,10 @@ size_t make_plan(Plan& p, int* nt, uint8_t* base) {
   p.gqa = p.a.n_heads / kv.n_kv_heads;
   p.rows = p.gqa * p.a.n_new;
   const uint32_t units = (p.a.max_len + pattn::UNIT - 1) / pattn::UNIT;
+  // A share is 4 units at least, and a sequence of up to 4 is not split. In calls of us at 2, 4 and 8, f32 over f16, 32/8 heads of
+  // 64: one sequence of 300 10.1, 13.3, 8.6 (unsplit), of 600 10.2, 12.6, 16.4, 16 of 500 14.6, 15.8, 14.9; bf16, 128 wide: one of 1024
+  // 11.9, 15.0, 16.9, four of 1000 15.4, 17.3, 21.4. (Smaller shares gain on one short sequence: more partial results, for which
+  // the workspace grows, and shorter ones.) Many or long sequences give every block more than that.
   p.min_units = 4;
   // 9 rows and more on the tcgen05 kernel, where its tiles fit: 64 or 128 wide heads, a tail of 15 positions at most, pages
   // that whole 8-row groups fill.

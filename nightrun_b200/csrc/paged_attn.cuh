@@ -27,8 +27,8 @@
 // 128-wide f16 heads) per warp in flight. (Pieces copied ahead into shared memory, 190 KB per SM in flight, were
 // slower: 248 against 199 us for 983 MB. It is the warps' instructions per tile that count, not the bytes in
 // flight.) For a few rows the rate of tcgen05 is not what is missing, and its tiles would have to pass through shared
-// memory. Measured: 64 sequences of 4096, 32/8 heads of 128, bf16: 174 us, 6.2 TB/s (0.95 of measured); 64 ragged ones up to
-// 16384: 158 us (0.96); one of 131072: 88 us and the join 8 us more (0.86).
+// memory. Measured: 64 sequences of 4096, 32/8 heads of 128, bf16: 168 us, 6.4 TB/s (0.98 of measured); 64 ragged ones up to
+// 16384: 161 us (0.94); one of 131072, f16: 88 us (0.94) and the join 8 us more.
 //
 // Split parts. The tensor cores take operands of the cache's type. q (scaled by a power of two to at most 2 per row) enters
 // as PARTS values of that type whose sum holds its bits: one where it is no wider than the cache, two bf16 for f16, three
@@ -154,8 +154,10 @@ NRC_DEV uint32_t seq_len(const Plan& p, uint32_t b) {
 NRC_DEV uint32_t units_of(uint32_t len, uint32_t unit = UNIT) { return len ? (len + unit - 1) / unit : 1u; }
 // What a (sequence, KV head, row block) costs its first block beside its units: the queries, the first tiles' latency, the
 // join. Counted in units, so that a share of many short sequences is not longer than one of a long sequence's middle (64
-// ragged sequences: 188 us uncounted, 158 us; the tcgen05 kernel on 24: 106 us at 6, 73 us at 14, 76 us at 20; its weights'
-// pass 39 us at 3, 35 us at 6, 37 us at 12).
+// ragged sequences: 188 us uncounted, 158 us). On tcgen05, 24 sequences of 1000..9001, 5 new tokens, calls of us at 6, 14 and
+// 20 units, then what the weights' pass adds at 3, 6 and 12: 40/8 heads of 64, f32 over f16 99, 92, 96 and 54, 45, 45; bf16 102, 101, 101
+// and 49, 44, 52; 32/8 heads of 128, f16 133, 137, 137 and 75, 65, 72; f32 over bf16 146, 147, 147 and 79, 71, 73; 64 of 300..4000 with 4 new
+// tokens, bf16 167, 173, 188 and 124, 89, 88. Wide heads' tiles cost more each, so they would do with fewer.
 constexpr uint32_t SETUP = 2, TC_SETUP = 14, TC_WEIGHTS_SETUP = 6;
 constexpr int TC_TILE = 128;         // rows of a tile of the tcgen05 kernel
 
@@ -825,8 +827,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ P
   if (d == 0 && p.lse) p.lse[((size_t)b * p.a.kv.n_kv_heads + h) * p.rows + r] = log2f(sum) - low;
 }
 
-// Weights: the scores again (the same products, the same bits; they would take more memory traffic than K does), then
-// 2^(s - lse) summed over the query rows in a fixed order and added. The attention's schedule, without row blocks.
+// Weights: the scores again (the same products, the same bits), then 2^(s - lse) summed over the query rows in a fixed order and
+// added. The attention's schedule, without row blocks. Bound by reading K again, 95 us beside the attention's 168 for 64
+// sequences of 4096, 32/8 heads of 128, bf16. (Scores kept by the attention would be 8 bytes per row and position, written and
+// read, where K is 2 per value: less below head_dim / 4 rows, more from there on. Not built; it takes a workspace of the
+// positions' size.)
 template <bool BF, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(THREADS, WEIGHTS_RESIDENT) k_weights(const __grid_constant__ Plan p) {
   constexpr int COLS = 8 * NT;

@@ -12,9 +12,10 @@
 // of four softmax warps take turns at the tiles, each with its own scores, weights, references and accumulators (joined at
 // the end), so that one computes while the other's products run.
 //
-// Measured, this kernel against mma.sync: 24 sequences of 1000..9001, 40/8 heads of 64, 5 new tokens, f32 over f16: 75
-// against 99 us; 16 of 4096, 32/8 heads of 128, f16: 8 new tokens 76 against 121 us, 4 new tokens 70 against 74 us (3.9
-// TB/s). The weights' pass, 24 sequences as above: 35 against 60 us, part of it under the join. A piece of work costs some 14
+// Measured, calls with the join, this kernel against mma.sync: 16 sequences of 4096, 12, 16, 24 and 32 rows: f16, 64 wide 37, 56,
+// 60, 63 against 35, 58, 76, 80 us, 128 wide 49, 77, 82, 86 against 49, 78, 129, 136 us; f32 over f16, 128 wide 50, 78, 84, 88 against 52, 84,
+// 158, 166 us; f32 over bf16 54, 84, 90, 94 against 57, 93, 178, 185 us. 24 sequences of 1000..9001, 40/8 heads of 64, 5 new tokens, f32
+// over f16: 92 against 138 us, with weights 137 against 193 us. A piece of work costs some 14
 // tiles beside its tiles (queries in, the pipeline filled and drained, the tail, the join), which is what bounds it now where
 // sequences are short; the schedule counts them.
 //
