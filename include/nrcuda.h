@@ -211,7 +211,7 @@ int nrc_rope_append(const nrc_paged_kv* kv, const nrc_rope_args* args, void* str
  * counts the cached positions, the new tokens' own among them; token i of n_new sees the positions
  * before lens[s] - (n_new - 1 - i); one that sees nothing gets zeros. Per query head
  *   out = sum_t p_t V_t,  p = softmax(scale * q . K_t),
- * infinite keys and values as in f32: a score of -inf has weight 0, one of +inf or NaN makes its row NaN, an infinite value of
+ * infinite keys and values as in f32: a score of -inf has weight 0 (zeros for a row of nothing else), one of +inf or NaN makes its row NaN, an infinite value of
  * weight above 0 is the output's; rows that do not see them are unharmed (they cost such a row a slower pass);
  * dots, softmax and sums in f32. Tensor cores form the products: q and p enter them split into parts of the cache's type. q
  * whole, but f32 over f16 in 22 bits below its row's largest value; p in 22 bits (f16) or 16 (bf16; f32 calls 24), however wide

@@ -47,6 +47,7 @@ constexpr uint32_t tc_drain(bool bf, int parts) { return parts == (bf ? 3 : 2) ?
 // products of tile T - 1 - D are done (in the weights' pass, where only K goes through the ring of D), hence that the scores
 // two tiles before that have been read, and the masks with them. T - 2 - D may still be waiting to be: D + 3 at least.
 constexpr int TC_MASKS = 16;
+constexpr float TC_UNSEEN = -3.40282347e38f;  // among the tail's scores: of a position that the row does not see
 constexpr int TC_COLS = 32, TC_THREADS = 10 * 32, TC_SOFTMAX = 256;
 constexpr int tc_half(int hd) { return TC_TILE * hd * 2; }  // bytes of a half stage: one tile of K or V
 constexpr int tc_ring(int hd, int parts) { return hd == 64 ? 6 : parts < 3 ? 5 : 4; }
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
       if (tail) {
         for (uint32_t i = threadIdx.x; i < TC_COLS * tail; i += TC_SOFTMAX) {
           const uint32_t c = i / tail, j = i - c * tail, r = w.rb * TC_COLS + c, tok = r / p.gqa;
-          float x = -INFINITY;
+          float x = TC_UNSEEN;
           if (r < p.rows && w.seen + j + (p.a.n_new - 1 - tok) < w.len && tail_off[j] >= 0) {
             const uint4* kr = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a.kv.k) + tail_off[j]);
             x = dot_row<BF, HD>(p, query_row(p, w.b, w.h, r), kr) * (p.a.scale * 1.44269504088896340736f);
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
           float sum = 0.0f;
           for (int c = 0; c < TC_COLS; c++) {
             const float t = tail_s[c][threadIdx.x];
-            if (t != -INFINITY) sum += exp2_fast(t + ref_s[0][c]);
+            if (t != TC_UNSEEN) sum += exp2_fast(t + ref_s[0][c]);
           }
           if (tail_off[threadIdx.x] >= 0)
             p.a.weights[((size_t)w.b * p.a.kv.n_kv_heads + w.h) * p.a.weights_len + w.seen + threadIdx.x] += sum;
@@ -649,9 +650,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         float sum = f0 * (l_s[0][0][c] + l_s[0][1][c] + l_s[0][2][c] + l_s[0][3][c]) +
                     f1 * (l_s[1][0][c] + l_s[1][1][c] + l_s[1][2][c] + l_s[1][3][c]);
         for (uint32_t j = 0; j < tail; j++) {
-          const float x = tail_s[c][j], e = x == -INFINITY ? 0.0f : exp2_fast(x + low);
-          tail_s[c][j] = x == -INFINITY ? -1.0f : e;  // not seen: not even 0 times what stands there
-          sum += e;
+          const float x = tail_s[c][j], e = exp2_fast(x + low);
+          tail_s[c][j] = x == TC_UNSEEN ? -1.0f : e;  // not seen: not even 0 times what stands there
+          if (x != TC_UNSEEN) sum += e;
         }
         f_s[0][c] = f0;
         f_s[1][c] = f1;

@@ -245,6 +245,43 @@ def test_infinite_and_nan_keys_reach_their_rows_only(K, case):
     same(w, ww, wtol + 1e-30)
 
 
+@pytest.mark.parametrize("case", [ODD[1], ODD[5], ODD[6], ODD[8]], ids=["unsplit", "mma", "tcgen05 64", "tcgen05 128"])
+def test_scores_of_minus_infinity_count_alike_everywhere(K, case):
+    """A score of -inf among the newest positions, which only some tokens see, as anywhere else: 0 times an infinite value is
+    NaN, and in a row that is NaN the position's weight is too."""
+    q, k, v, table, lens = odd_case(K, case, 36)
+    q[..., 5] = -q[..., 5].abs().clamp(min=0.01)
+    for s, n in enumerate(lens.tolist()):
+        for t in (n - 2, n // 2):
+            row = R.rows(k, table, s, [t])[0].clone()
+            row[:, 5] = INF
+            R.put(k, table, s, t, row)
+        row = R.rows(v, table, s, [n - 2])[0].clone()
+        row[0, 9] = INF
+        R.put(v, table, s, n - 2, row)
+        row = R.rows(k, table, s, [3])[0].clone()
+        row[1, 7] = NAN
+        R.put(k, table, s, 3, row)
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.2)
+    out, w = run_odd(K, q, k, v, table, lens, 0.2)
+    same(out, want, tol)
+    same(w, ww, wtol + 1e-30)
+
+
+@pytest.mark.parametrize("case", ODD, ids=[str(i) for i in range(len(ODD))])
+def test_rows_of_nothing_but_minus_infinity_get_zeros(K, case):
+    """Every score of a KV head's rows is -inf: zeros, as where a row sees nothing, and no weight."""
+    q, k, v, table, lens = odd_case(K, case, 37)
+    g = q.shape[2] // k.shape[2]
+    q[:, :, :g, 5] = -q[:, :, :g, 5].abs().clamp(min=0.01)
+    k[:, :, 0, 5] = INF
+    out, w = run_odd(K, q, k, v, table, lens, 0.2)
+    assert not out[:, :, :g].any() and not w[:, 0].any()
+    want, tol, ww, wtol = expected(q, k, v, table, lens, 0.2)
+    same(out[:, :, g:], want[:, :, g:], tol[:, :, g:])
+    same(w[:, 1:], ww[:, 1:], wtol[:, 1:] + 1e-30)
+
+
 @pytest.mark.parametrize("case", [ODD[1], ODD[6]], ids=["few", "many"])
 def test_nan_queries_reach_their_rows_only(K, case):
     q, k, v, table, lens = odd_case(K, case, 34)
